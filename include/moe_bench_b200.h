@@ -331,6 +331,100 @@ int mb200_set_comm_only(int enabled);
  * (0 = no kernel gave up a wait).  Not capturable. */
 int mb200_read_status(const void* workspace, int32_t* status_out, void* stream);
 
+/* ---- products and norms around the expert FFN, forward and backward ----
+ *
+ * What a training or serving program runs next to the layer forward: the plain product over the
+ * experts' ragged row segments with its gradients, a dense product with bias, activation and
+ * residual (gate projection, shared expert) with its gradients, and layer norm with its
+ * gradients.  The reference has none of them (it draws routing directly, data.py:178-235, and
+ * times forwards only); the definitions are the formulas given here.
+ *
+ * Common rules
+ *  - precision: MB200_PRECISION_BF16 or _FP16, the type of every tensor not said to be another;
+ *    products are summed in fp32 and rounded once, to the output's type;
+ *  - a matrix is row-major with its columns side by side and `pitch` elements from row to row;
+ *    the operands of products (x, w, and dy unless it has to be copied, see there) start on a
+ *    16-byte boundary and have pitches that are multiples of 8 elements, and k is a multiple
+ *    of 8; n, rows and segment lengths are any; outputs are dense (pitch = columns);
+ *  - calls that share no output and no workspace may overlap; a workspace (16-byte aligned, no
+ *    initial contents needed) is free again when the call's work on the stream is done;
+ *  - results do not depend on what else runs: every sum has a fixed order;
+ *  - an in-kernel wait that expires (4 s) leaves 100 + site in this device's status word of the
+ *    library, which mb200_linear_status reads. */
+#define MB200_ACT_NONE 0
+#define MB200_ACT_RELU 1
+#define MB200_ACT_SILU 2      /* z / (1 + exp(-z)) */
+#define MB200_ACT_GELU 3      /* z * (1 + erf(z / sqrt 2)) / 2 */
+#define MB200_ACT_GELU_TANH 4 /* z * (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
+
+/* y = act(z) + residual, z = x . w^T + bias, for x [rows, k], w [n, k]; bias [n] (fp32 if
+ * bias_fp32, else the precision's type) or NULL; residual [rows, n] or NULL; y [rows, n], fp32
+ * if out_fp32.  slope: NULL, or [rows, n] in the precision's type that receives act'(z), the
+ * one thing of the forward that the backward call below needs besides x and w.  y may be the
+ * residual's buffer (same type and pitch n). */
+int64_t mb200_linear_workspace_bytes(int64_t rows, int n, int k, int device);
+int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, const void* w, int64_t w_pitch,
+                 int n, int k, const void* bias, int bias_fp32, int activation, const void* residual,
+                 int64_t residual_pitch, void* y, int out_fp32, void* slope, void* workspace,
+                 int64_t workspace_bytes, int device, void* stream);
+
+/* Gradients of mb200_linear (the residual's is dy itself).  dz = dy * slope (slope NULL: dz = dy):
+ * dx = dz . w [rows, k]; dw = dz^T . x [n, k], fp32 if dw_fp32; db = sum of dz over the rows, fp32
+ * [n], from dz before any rounding.  Each of dx, dw, db may be NULL.  dy [rows, n] is fp32 if
+ * dy_fp32 (bf16 only: the range of fp16 does not hold such a gradient).  The products take dz in
+ * the precision's type: where slope is given or dy is fp32 it is rounded to it once, into the
+ * workspace, and a dy that breaks the alignment rules (n odd, say) is copied there too. */
+int64_t mb200_linear_backward_workspace_bytes(int64_t rows, int n, int k, int device);
+int mb200_linear_backward(int precision, const void* dy, int dy_fp32, int64_t dy_pitch, const void* slope,
+                          const void* x, int64_t x_pitch, int64_t rows, const void* w, int64_t w_pitch, int n,
+                          int k, void* dx, void* dw, int dw_fp32, float* db, void* workspace,
+                          int64_t workspace_bytes, int device, void* stream);
+
+/* y[r, :] = x[r, :] . w[e]^T for the rows r of segment e: offsets [experts + 1] int32 in device
+ * memory, ascending, segment e = rows offsets[e] .. offsets[e+1] - 1, any length from zero up.
+ * These are mtile_prefix of mb200_align at pad_rows = 1, whose sorted_ids then are the rows'
+ * assignments.  w [experts, n, k] with w_expert_pitch elements from expert to expert (a multiple
+ * of 8).  Rows of y outside the segments are left as they were; offsets beyond the rows are cut
+ * to them, and a segment that ends before it begins is empty. */
+int mb200_grouped_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, const void* w,
+                         int64_t w_pitch, int64_t w_expert_pitch, const int32_t* offsets, int experts, int n,
+                         int k, void* y, int device, void* stream);
+
+/* Gradients of mb200_grouped_linear: dx[r, :] = dy[r, :] . w[e] (rows outside the segments left
+ * as they were), dw[e] = sum over the rows of segment e of dy[r]^T x[r], [experts, n, k] dense,
+ * fp32 if dw_fp32, zero for an empty segment.  dx or dw may be NULL; rows outside the segments,
+ * whatever they hold, have no part in any result.  The workspace holds a copy of a dy that
+ * breaks the alignment rules; else it may be NULL. */
+int64_t mb200_grouped_linear_backward_workspace_bytes(int64_t rows, int n);
+int mb200_grouped_linear_backward(int precision, const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch,
+                                  int64_t rows, const void* w, int64_t w_pitch, int64_t w_expert_pitch,
+                                  const int32_t* offsets, int experts, int n, int k, void* dx, void* dw,
+                                  int dw_fp32, void* workspace, int64_t workspace_bytes, int device, void* stream);
+
+/* The status word of the calls above on the current device, after synchronising `stream`
+ * (0 = no wait expired); clear != 0 sets it back to 0.  Not capturable. */
+int mb200_linear_status(int32_t* status_out, int clear, void* stream);
+
+/* Layer norm over the last dimension: mean and rstd = 1 / sqrt(variance + eps) of every row in
+ * fp32 (variance about the mean, divided by hidden), y = (x - mean) * rstd * weight + bias.
+ * x [rows, hidden], y [rows, hidden] dense; weight, bias [hidden] or NULL.  precision also takes
+ * MB200_PRECISION_FP32 here, the type of x, y, weight and bias alike; params_fp32: weight and
+ * bias are fp32 whatever x is.  Any hidden from 1 up, any pitch >= hidden. */
+#define MB200_PRECISION_FP32 3
+int mb200_layer_norm(int precision, const void* x, int64_t x_pitch, int64_t rows, int64_t hidden, const void* weight,
+                     const void* bias, int params_fp32, float eps, void* y, float* mean, float* rstd, int device,
+                     void* stream);
+
+/* Gradients of mb200_layer_norm.  With h = (x - mean) * rstd and g = dy * weight:
+ * dx = rstd * (g - mean over the row of g - h * mean over the row of g*h), in x's type;
+ * dweight = sum over the rows of dy * h, dbias = sum over the rows of dy, both fp32 [hidden].
+ * Each of dx, dweight, dbias may be NULL. */
+int64_t mb200_layer_norm_backward_workspace_bytes(int64_t rows, int64_t hidden, int device);
+int mb200_layer_norm_backward(int precision, const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch,
+                              int64_t rows, int64_t hidden, const float* mean, const float* rstd,
+                              const void* weight, int params_fp32, void* dx, float* dweight, float* dbias,
+                              void* workspace, int64_t workspace_bytes, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

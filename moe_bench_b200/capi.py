@@ -20,6 +20,7 @@ ABI_VERSION = 5
 PRECISION_BF16 = 0
 PRECISION_FP8 = 1
 PRECISION_FP16 = 2
+PRECISION_FP32 = 3
 PAD_ROWS_BF16 = 16
 PAD_ROWS_FP8 = 128
 
@@ -84,6 +85,39 @@ SIGNATURES = {
     "mb200_set_fp8_scale_format": (c_i32, [c_i32]),
     "mb200_set_comm_only": (c_i32, [c_i32]),
     "mb200_read_status": (c_i32, [c_vp, c_vp, c_vp]),
+    "mb200_linear_workspace_bytes": (c_i64, [c_i64, c_i32, c_i32, c_i32]),
+    "mb200_linear": (
+        c_i32,
+        [c_i32, c_vp, c_i64, c_i64, c_vp, c_i64, c_i32, c_i32, c_vp, c_i32, c_i32, c_vp, c_i64, c_vp, c_i32, c_vp,
+         c_vp, c_i64, c_i32, c_vp],
+    ),
+    "mb200_linear_backward_workspace_bytes": (c_i64, [c_i64, c_i32, c_i32, c_i32]),
+    "mb200_linear_backward": (
+        c_i32,
+        [c_i32, c_vp, c_i32, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_i32, c_vp,
+         c_vp, c_i64, c_i32, c_vp],
+    ),
+    "mb200_grouped_linear": (
+        c_i32,
+        [c_i32, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i32, c_i32, c_i32, c_vp, c_i32, c_vp],
+    ),
+    "mb200_grouped_linear_backward_workspace_bytes": (c_i64, [c_i64, c_i32]),
+    "mb200_grouped_linear_backward": (
+        c_i32,
+        [c_i32, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i32, c_i32, c_i32, c_vp, c_vp, c_i32,
+         c_vp, c_i64, c_i32, c_vp],
+    ),
+    "mb200_linear_status": (c_i32, [c_vp, c_i32, c_vp]),
+    "mb200_layer_norm": (
+        c_i32,
+        [c_i32, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i32, ctypes.c_float, c_vp, c_vp, c_vp, c_i32, c_vp],
+    ),
+    "mb200_layer_norm_backward_workspace_bytes": (c_i64, [c_i64, c_i64, c_i32]),
+    "mb200_layer_norm_backward": (
+        c_i32,
+        [c_i32, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_i64,
+         c_i32, c_vp],
+    ),
 }
 
 
@@ -468,3 +502,273 @@ def read_kernel_clocks(workspace: torch.Tensor) -> dict:
     for name, (cyc, ns) in (("gate_up_gemm", vals[0:2]), ("down_gemm", vals[2:4])):
         out[name] = None if ns <= 0 else round(cyc / ns * 1e3, 1)
     return out
+
+
+# ---- products and norms around the expert FFN ----
+# The tensors of these calls may be on any device: the call runs there, on that device's current stream.
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+_H16 = {torch.bfloat16: PRECISION_BF16, torch.float16: PRECISION_FP16}
+_NORM_TYPES = {**_H16, torch.float32: PRECISION_FP32}
+
+
+def _h16(t: torch.Tensor, name: str) -> int:
+    if not t.is_cuda:
+        raise MB200Error(f"{name}: need a CUDA tensor, got one on {t.device}; there is no CPU path")
+    if t.dtype not in _H16:
+        raise MB200Error(f"{name}: need bf16 or fp16, got {t.dtype}")
+    return _H16[t.dtype]
+
+
+def _pitch(t: torch.Tensor, like: torch.Tensor, shape, name: str, dtypes=None) -> int:
+    """Elements from row to row of a matrix whose columns lie side by side; refuses every other layout."""
+    dtypes = (like.dtype,) if dtypes is None else dtypes
+    if t.dtype not in dtypes or t.device != like.device:
+        raise MB200Error(f"{name}: need {' or '.join(map(str, dtypes))} on {like.device}, got {t.dtype} on {t.device}")
+    if tuple(t.shape) != tuple(shape):
+        raise MB200Error(f"{name}: need shape {tuple(shape)}, got {tuple(t.shape)}")
+    rows, cols = shape[-2:]
+    if cols != 1 and t.stride(-1) != 1:
+        raise MB200Error(f"{name}: the elements of a row must lie side by side, got strides {t.stride()}")
+    if rows <= 1:
+        return (cols + 7) // 8 * 8  # the stride of a single row says nothing
+    if t.stride(-2) < cols:
+        raise MB200Error(f"{name}: rows overlap (strides {t.stride()})")
+    return t.stride(-2)
+
+
+def _vector(t: Optional[torch.Tensor], like: torch.Tensor, n: int, name: str, dtypes) -> None:
+    if t is None:
+        return
+    if t.dtype not in dtypes or t.device != like.device or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise MB200Error(f"{name}: need a contiguous vector of {n} elements of {' or '.join(map(str, dtypes))} on "
+                         f"{like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _output(t: Optional[torch.Tensor], like: torch.Tensor, shape, dtype, name: str) -> torch.Tensor:
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if t.dtype != dtype or t.device != like.device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise MB200Error(f"{name}: need a contiguous tensor of {dtype} {tuple(shape)} on {like.device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    return t
+
+
+def _scratch(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    if nbytes < 0:
+        raise MB200Error(load().mb200_last_error().decode())
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+class _on_device:
+    """Makes a tensor's device the current one for a call."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, t: torch.Tensor) -> None:
+        self.index = t.device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, out_dtype=None, want_slope: bool = False):
+    """``act(x @ w.T + bias) + residual`` for ``x [rows, k]``, ``w [n, k]`` of bf16 or fp16, summed in fp32 and rounded
+    once.  ``bias [n]`` may be fp32; ``activation``: one of ``ACTIVATIONS``; ``out_dtype``: x's type or ``torch.float32``.
+    Rows may be further apart than they are long (a multiple of 8 elements); ``k`` is a multiple of 8, ``n`` is free.
+    ``out`` may be the residual itself.  With ``want_slope`` also returns ``act'(x @ w.T + bias)`` in x's type, which
+    ``linear_backward`` takes."""
+    precision = _h16(x, "x")
+    if x.dim() != 2 or w.dim() != 2:
+        raise MB200Error(f"linear: need matrices, got x {tuple(x.shape)} and w {tuple(w.shape)}")
+    rows, k = x.shape
+    n = w.shape[0]
+    if activation not in ACTIVATIONS:
+        raise MB200Error(f"activation {activation!r}: expected one of {sorted(ACTIVATIONS)}")
+    xp, wp = _pitch(x, x, (rows, k), "x"), _pitch(w, x, (n, k), "w")
+    _vector(bias, x, n, "bias", (x.dtype, torch.float32))
+    rp = _pitch(residual, x, (rows, n), "residual") if residual is not None else 0
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise MB200Error(f"linear: output of {out_dtype} for operands of {x.dtype}")
+    y = _output(out, x, (rows, n), out_dtype, "out")
+    slope = torch.empty((rows, n), dtype=x.dtype, device=x.device) if want_slope else None
+    lib = load()
+    with _on_device(x):
+        ws = _scratch(lib.mb200_linear_workspace_bytes(rows, n, k, x.device.index), x)
+        _check(
+            lib.mb200_linear(
+                precision, _ptr(x), xp, rows, _ptr(w), wp, n, k, _ptr(bias), bias is not None and bias.dtype == torch.float32,
+                ACTIVATIONS[activation], _ptr(residual), rp, _ptr(y), out_dtype == torch.float32, _ptr(slope), _ptr(ws),
+                0 if ws is None else ws.numel(), x.device.index, _stream(x.device),
+            ),
+            "linear",
+        )
+    return (y, slope) if want_slope else y
+
+
+def _dw_type(w: torch.Tensor, dw_dtype):
+    dw_dtype = w.dtype if dw_dtype is None else dw_dtype
+    if dw_dtype not in (w.dtype, torch.float32):
+        raise MB200Error(f"weight gradient of {dw_dtype} for weights of {w.dtype}")
+    return dw_dtype
+
+
+def linear_backward(dy, x, w, slope=None, dw_dtype=None, want_dx: bool = True, want_dw: bool = True, want_db: bool = True):
+    """Gradients ``(dx, dw, db)`` of ``linear`` (None where not wanted; the residual's gradient is ``dy``).  ``slope``: what
+    ``linear(..., want_slope=True)`` returned, None for no activation.  ``dy`` may be fp32 for bf16 operands.  ``dy * slope``
+    is rounded to x's type once, for the products; ``db`` is its fp32 sum before that; ``dw`` has w's type, or fp32."""
+    precision = _h16(x, "x")
+    if x.dim() != 2 or w.dim() != 2:
+        raise MB200Error(f"linear_backward: need matrices, got x {tuple(x.shape)} and w {tuple(w.shape)}")
+    rows, k = x.shape
+    n = w.shape[0]
+    xp, wp = _pitch(x, x, (rows, k), "x"), _pitch(w, x, (n, k), "w")
+    types = (x.dtype, torch.float32) if x.dtype == torch.bfloat16 else (x.dtype,)
+    dp = _pitch(dy, x, (rows, n), "dy", types)
+    if slope is not None:
+        _output(slope, x, (rows, n), x.dtype, "slope")
+    dw_dtype = _dw_type(w, dw_dtype)
+    dx = torch.empty((rows, k), dtype=x.dtype, device=x.device) if want_dx else None
+    dw = torch.empty((n, k), dtype=dw_dtype, device=x.device) if want_dw else None
+    db = torch.empty(n, dtype=torch.float32, device=x.device) if want_db else None
+    lib = load()
+    with _on_device(x):
+        ws = _scratch(lib.mb200_linear_backward_workspace_bytes(rows, n, k, x.device.index), x)
+        _check(
+            lib.mb200_linear_backward(
+                precision, _ptr(dy), dy.dtype == torch.float32, dp, _ptr(slope), _ptr(x), xp, rows, _ptr(w), wp, n, k,
+                _ptr(dx), _ptr(dw), dw_dtype == torch.float32, _ptr(db), _ptr(ws), 0 if ws is None else ws.numel(),
+                x.device.index, _stream(x.device),
+            ),
+            "linear_backward",
+        )
+    return dx, dw, db
+
+
+def _expert_weight(w: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor):
+    """(experts, n, k, elements from row to row, from expert to expert)"""
+    if x.dim() != 2 or w.dim() != 3:
+        raise MB200Error(f"need x [rows, k] and w [experts, n, k], got {tuple(x.shape)} and {tuple(w.shape)}")
+    e, n, k = w.shape
+    wp = _pitch(w, x, (e, n, x.shape[1]), "w")
+    ep = w.stride(0) if e > 1 else (n * wp + 7) // 8 * 8
+    if ep < n * wp - (wp - k) and e > 1:
+        raise MB200Error(f"w: experts overlap (strides {w.stride()})")
+    _vector(offsets, x, e + 1, "offsets", (torch.int32,))
+    return e, n, k, wp, ep
+
+
+def grouped_linear(x, w, offsets, out=None):
+    """``x[r] @ w[e].T`` for the rows of segment e = ``offsets[e] .. offsets[e + 1] - 1``, of any length: x [rows, k] and
+    w [experts, n, k] of bf16 or fp16, offsets [experts + 1] int32 on x's device (``align(..., pad_rows=1)`` returns them as
+    ``mtile_prefix``).  Rows outside the segments are left as they are in ``out``, undefined in a tensor made here."""
+    precision = _h16(x, "x")
+    e, n, k, wp, ep = _expert_weight(w, x, offsets)
+    rows = x.shape[0]
+    xp = _pitch(x, x, (rows, k), "x")
+    y = _output(out, x, (rows, n), x.dtype, "out")
+    with _on_device(x):
+        _check(
+            load().mb200_grouped_linear(precision, _ptr(x), xp, rows, _ptr(w), wp, ep, _ptr(offsets), e, n, k, _ptr(y),
+                                        x.device.index, _stream(x.device)),
+            "grouped_linear",
+        )
+    return y
+
+
+def grouped_linear_backward(dy, x, w, offsets, dw_dtype=None, dx_out=None, want_dx: bool = True, want_dw: bool = True):
+    """Gradients ``(dx, dw)`` of ``grouped_linear`` (None where not wanted).  Rows outside the segments have no part in
+    ``dw`` and are left as they are in ``dx_out``; an expert without rows gets a zero gradient.  ``dw`` has w's type, or fp32."""
+    precision = _h16(x, "x")
+    e, n, k, wp, ep = _expert_weight(w, x, offsets)
+    rows = x.shape[0]
+    xp, dp = _pitch(x, x, (rows, k), "x"), _pitch(dy, x, (rows, n), "dy")
+    dw_dtype = _dw_type(w, dw_dtype)
+    dx = _output(dx_out, x, (rows, k), x.dtype, "dx_out") if want_dx else None
+    dw = torch.empty((e, n, k), dtype=dw_dtype, device=x.device) if want_dw else None
+    lib = load()
+    with _on_device(x):
+        copied = dp % 8 or dy.data_ptr() % 16
+        ws = _scratch(lib.mb200_grouped_linear_backward_workspace_bytes(rows, n), x) if copied else None
+        _check(
+            lib.mb200_grouped_linear_backward(
+                precision, _ptr(dy), dp, _ptr(x), xp, rows, _ptr(w), wp, ep, _ptr(offsets), e, n, k, _ptr(dx), _ptr(dw),
+                dw_dtype == torch.float32, _ptr(ws), 0 if ws is None else ws.numel(), x.device.index, _stream(x.device),
+            ),
+            "grouped_linear_backward",
+        )
+    return dx, dw
+
+
+def linear_status(device=None, clear: bool = False) -> int:
+    """Synchronise the device's current stream and return the status word of the products above (0 = every in-kernel wait
+    completed); ``clear`` sets it back to 0."""
+    val = ctypes.c_int32(0)
+    with torch.cuda.device(device):
+        _check(load().mb200_linear_status(ctypes.byref(val), 1 if clear else 0, _stream(device)), "linear_status")
+    return int(val.value)
+
+
+def _norm_operands(x, weight, bias, name: str):
+    if not x.is_cuda:
+        raise MB200Error(f"{name}: need CUDA tensors, got one on {x.device}; there is no CPU path")
+    if x.dtype not in _NORM_TYPES:
+        raise MB200Error(f"{name}: need bf16, fp16 or fp32, got {x.dtype}")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise MB200Error(f"{name}: need x [rows, hidden], got {tuple(x.shape)}")
+    h = x.shape[1]
+    types = {t.dtype for t in (weight, bias) if t is not None}
+    if len(types) > 1:
+        raise MB200Error(f"{name}: weight and bias of one type, got {sorted(map(str, types))}")
+    for t, what in ((weight, "weight"), (bias, "bias")):
+        _vector(t, x, h, what, (x.dtype, torch.float32))
+    return _NORM_TYPES[x.dtype], x.shape[0], h, types == {torch.float32}
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
+    """Layer norm of the rows of ``x [rows, hidden]`` (bf16, fp16 or fp32; rows may be any distance apart): returns
+    ``(y, mean, rstd)``, the last two in fp32 for ``layer_norm_backward``.  weight and bias have x's type or fp32."""
+    precision, rows, h, fp32 = _norm_operands(x, weight, bias, "layer_norm")
+    xp = _pitch(x, x, (rows, h), "x")
+    y = _output(out, x, (rows, h), x.dtype, "out")
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    mean, rstd = stats[0], stats[1]
+    with _on_device(x):
+        _check(
+            load().mb200_layer_norm(precision, _ptr(x), xp, rows, h, _ptr(weight), _ptr(bias), fp32, eps, _ptr(y), _ptr(mean),
+                                    _ptr(rstd), x.device.index, _stream(x.device)),
+            "layer_norm",
+        )
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
+    """Gradients ``(dx, dweight, dbias)`` of ``layer_norm`` (None where not wanted); the last two are fp32 sums over the rows,
+    in a fixed order."""
+    precision, rows, h, fp32 = _norm_operands(x, weight, None, "layer_norm_backward")
+    xp, dp = _pitch(x, x, (rows, h), "x"), _pitch(dy, x, (rows, h), "dy")
+    for t, what in ((mean, "mean"), (rstd, "rstd")):
+        _vector(t, x, rows, what, (torch.float32,))
+    dx = torch.empty((rows, h), dtype=x.dtype, device=x.device) if want_dx else None
+    dweight = torch.empty(h, dtype=torch.float32, device=x.device) if want_dweight else None
+    dbias = torch.empty(h, dtype=torch.float32, device=x.device) if want_dbias else None
+    lib = load()
+    with _on_device(x):
+        ws = None
+        if want_dweight or want_dbias:
+            ws = _scratch(lib.mb200_layer_norm_backward_workspace_bytes(rows, h, x.device.index), x)
+        _check(
+            lib.mb200_layer_norm_backward(
+                precision, _ptr(dy), dp, _ptr(x), xp, rows, h, _ptr(mean), _ptr(rstd), _ptr(weight), fp32, _ptr(dx),
+                _ptr(dweight), _ptr(dbias), _ptr(ws), 0 if ws is None else ws.numel(), x.device.index, _stream(x.device),
+            ),
+            "layer_norm_backward",
+        )
+    return dx, dweight, dbias
