@@ -99,6 +99,28 @@ int make_tensor_map_2d(CUtensorMap* map, const void* base, int elem_bytes, uint6
   return kOk;
 }
 
+int make_tensor_map_3d(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t groups, uint64_t row_bytes,
+                       uint64_t group_bytes, uint32_t box_rows, int fp16) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  MB200_REQUIRE(fn != nullptr, kDriverEntryMissing, "cuTensorMapEncodeTiled is not available");
+  if (groups == 1) group_bytes = rows * row_bytes;
+  MB200_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0 && row_bytes % 16 == 0 && group_bytes % 16 == 0, kInvalidArgument,
+                "tensor map: base address and strides must be multiples of 16 bytes");
+  const uint64_t most = uint64_t(1) << 40;
+  MB200_REQUIRE(row_bytes < most && (groups == 1 || group_bytes < most), kUnsupportedShape, "tensor map: strides of %llu and %llu bytes",
+                (unsigned long long)row_bytes, (unsigned long long)group_bytes);
+  if (group_bytes >= most) group_bytes = row_bytes;  // one group: never stepped over
+  const cuuint64_t dims[3] = {cols, rows, groups};
+  const cuuint64_t strides[2] = {row_bytes, group_bytes};
+  const cuuint32_t box[3] = {64, box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  MB200_REQUIRE(r == CUDA_SUCCESS, kCudaError, "cuTensorMapEncodeTiled failed with code %d", int(r));
+  return kOk;
+}
+
 // ---------------------------------------------------------------------------
 // Workspace layout
 // ---------------------------------------------------------------------------

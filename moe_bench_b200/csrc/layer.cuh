@@ -277,5 +277,9 @@ void mark_stage(int i, cudaStream_t s);
 // box_rows x (128 bytes of columns), 128-byte swizzle.
 int make_tensor_map_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t rows,
                        uint64_t cols, uint32_t box_rows, int fp16 = 0);
+// 3-D tensor of 16-bit elements, boxes of 1 x box_rows x 64 elements, 128-byte swizzle.  group_bytes is not
+// looked at where there is one group.
+int make_tensor_map_3d(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t groups, uint64_t row_bytes,
+                       uint64_t group_bytes, uint32_t box_rows, int fp16);
 
 }  // namespace mb200

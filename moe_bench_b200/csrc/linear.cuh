@@ -89,6 +89,22 @@ __device__ __forceinline__ float activate(int act, float z, float& slope) {
   }
 }
 
+// `residual` may be `out`: no promise that it is constant.
+struct Bias4 {
+  float v[4];
+};
+__device__ __forceinline__ Bias4 load_bias4(const Epilogue& e, int m, int f) {
+  Bias4 b{};
+  if (e.bias)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (f + i < m) b.v[i] = e.bias_fp32 ? __ldg(reinterpret_cast<const float*>(e.bias) + f + i) : load_h16(e.bias, f + i, e.fp16);
+  return b;
+}
+__device__ __forceinline__ uint2 pack_h16x4(const float (&v)[4], int fp16) {
+  return make_uint2(pack_h16x2(v[0], v[1], fp16), pack_h16x2(v[2], v[3], fp16));
+}
+
 // One element.
 __device__ __forceinline__ void finish_element(const Epilogue& e, int m, int64_t row, int f, float z) {
   if (e.bias) z += e.bias_fp32 ? reinterpret_cast<const float*>(e.bias)[f] : load_h16(e.bias, f, e.fp16);
@@ -107,7 +123,43 @@ __device__ __forceinline__ void finish_element(const Epilogue& e, int m, int64_t
     reinterpret_cast<uint16_t*>(e.out)[row * m + f] = to_h16(y, e.fp16);
 }
 
+// Four features side by side, f a multiple of 4.  `vec`: every tensor takes them as one access (then m is a multiple of 4).
+__device__ __forceinline__ void finish4(const Epilogue& e, int m, int64_t row, int f, float (&z)[4], const Bias4& bias,
+                                        bool vec) {
+  if (!vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (f + i < m) finish_element(e, m, row, f + i, z[i]);
+    return;
+  }
+  float slope[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) z[i] += bias.v[i];
+  if (e.slope) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = activate<true>(e.act, z[i], slope[i]);
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(e.slope) + row * m + f) = pack_h16x4(slope, e.fp16);
+  } else if (e.act) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = activate<false>(e.act, z[i], slope[i]);
+  }
+  if (e.residual) {
+    const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(e.residual) + row * e.residual_pitch + f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] += load_h16(&r, i, e.fp16);
+  }
+  if (e.out_fp32)
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(e.out) + row * m + f) = make_float4(z[0], z[1], z[2], z[3]);
+  else
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(e.out) + row * m + f) = pack_h16x4(z, e.fp16);
+}
+
 // products.cu
-int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaStream_t stream);
+// Bytes of workspace that launch_product wants for a dense product (one group), 0 where its sums are not split.
+int64_t product_workspace_bytes(ProductKind kind, int rows, int m, int n, int k, int device);
+// status word of the products on the current device
+int product_status(int* status_out, int clear, cudaStream_t stream);
+int launch_product(ProductKind kind, const ProductArgs& args, void* workspace, int64_t workspace_bytes, int device,
+                   cudaStream_t stream);
 
 }  // namespace mb200

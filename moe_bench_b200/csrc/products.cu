@@ -1,4 +1,25 @@
-// The products around the expert FFN (linear.cuh): every output element is one dot product.
+// The products around the expert FFN (linear.cuh) on the sm_100a tensor cores: forward, input gradient
+// and weight gradient, dense or over ragged row segments.
+//
+// out[j][f] = sum over c of A(f, c) B(j, c): the features f, which lie side by side in the output, sit on the
+// accumulator's rows (tensor-memory lanes), the output rows j on its columns.  A pair of CTAs computes a tile of
+// 256 features x up to 256 output rows (any multiple of 32): each CTA holds 128 features and half of the output
+// rows of every 64-deep step, 32 KiB for 512 cycles of products, where a single CTA with the same
+// accumulator needs 48.  Row segments therefore cost what they hold, rounded up to 32.
+//
+// Operands come in as they lie in memory, no transposed copies: 128-byte-swizzled TMA boxes of 64 terms of the
+// sum x 16..128 rows where the terms lie side by side (w and x of the forward, dz of the input gradient), of 64
+// features x 64 terms where the features do (w of the input gradient, x and dz of the weight gradient).  Terms past
+// the end of a dense sum are the copy's zero fill.  A segment's last step in the weight gradient would read the next
+// segment's rows: those are overwritten with zeros in shared memory before the products read them, in both
+// operands, so that NaN and infinities there reach nothing.
+//
+// 384 threads: warp 0 loads, warp 1 of the pair's first CTA issues the products, warp 2 clears those tails,
+// warps 4-11 drain the accumulators (two sets, so that the next tile's products run meanwhile): 32 features x 16
+// output rows at a time go through a 2 KiB block of shared memory that turns them round, still in fp32, and leave
+// through the epilogue as 64 contiguous bytes per output row.  Every wait is bounded.
+
+#include <atomic>
 
 #include "linear.cuh"
 
@@ -6,74 +27,526 @@ namespace mb200 {
 
 namespace {
 
-constexpr int kTile = 64;   // features and output rows of a block's tile
-constexpr int kDepth = 16;  // terms of the sums per step
+constexpr int kThreads = 384;
+constexpr int kEpilogueWarps = 8;
+constexpr int kFirstEpilogueWarp = 4;
+constexpr int kMaxStages = 10;
+constexpr int kStep = 64;                 // terms of the sum per step
+constexpr int kABytes = 128 * 128;        // a CTA's 128 features of a step
+constexpr int kTileRows = 256;            // output rows of a tile at most
+constexpr int kTileFeatures = 256;
+constexpr int kBoxes = 4;                 // row boxes of 16, 32, 64, 128
+constexpr int kTmemCols = 512;
+constexpr int kBand = 8;                  // tiles that run side by side share 8 row blocks and as many feature blocks
 
-// 256 threads, 4 x 4 outputs each, operands staged in shared memory as fp32.
+struct SmemTail {
+  alignas(16) float turn[kEpilogueWarps][16 * 32];
+  uint64_t full[kMaxStages];    // of the pair's first CTA: a step of both CTAs has landed
+  uint64_t empty[kMaxStages];   // the products have read the stage
+  uint64_t raw[kMaxStages];     // weight gradient: this CTA's part of a segment's last step has landed
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];        // of the pair's first CTA
+  uint32_t tmem_base;
+  int abort_flag;
+  int max_len;                  // longest segment
+  int begin[kMaxExperts];
+  int len[kMaxExperts];
+  int blocks[kMaxExperts + 1];  // row blocks before each group
+};
+
+constexpr size_t kSmemLimit = 227 * 1024;
+constexpr size_t kRingBytes = (kSmemLimit - 1024 - sizeof(SmemTail)) / 1024 * 1024;
+constexpr size_t kSmemBytes = 1024 + kRingBytes + sizeof(SmemTail);
+static_assert(kRingBytes >= 6 * (kABytes + 128 * 128), "full tiles want six stages");
+
+struct Maps {
+  CUtensorMap a;
+  CUtensorMap b[kBoxes];
+};
+
+struct TileShape {
+  int f_tiles;      // feature blocks
+  int row_blocks;   // weight gradient: blocks of output rows per group
+  int splits;       // parts of every sum, each with a tile of its own
+  float* partial;   // [splits][output rows][partial_pitch] where splits > 1
+  int64_t partial_rows, partial_pitch;
+  int vec;          // the epilogue may access four features at once
+};
+
+// first failure of a wait, wait limit in ms, 0, 0
+__device__ int g_status[4];
+
+struct Tile {
+  int group, f0;
+  int64_t out_row;    // first output row
+  int b_row;          // its row coordinate in b (weight gradient: its column)
+  int cols, valid;    // output rows computed, and stored
+  int c_begin;        // weight gradient: first row of the segment
+  int depth;          // terms of the whole sum
+  int step0, step1;   // steps of this part
+  int split;
+};
+
 template <int kKind>
-__global__ void __launch_bounds__(256) product_kernel(const ProductArgs p) {
-  __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
-  const int group = blockIdx.z;
-  const int f0 = blockIdx.x * kTile;
-  int begin, end;
-  segment_of(p, group, begin, end);
-  const int count = kKind == kWeightGrad ? p.n : end - begin;   // output rows of the group
-  const int depth = kKind == kWeightGrad ? end - begin : p.k;
-  const int fp16 = p.epi.fp16;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int j0 = blockIdx.y * kTile; j0 < count; j0 += gridDim.y * kTile) {
-    float acc[4][4] = {};
-    for (int c0 = 0; c0 < depth; c0 += kDepth) {
-      for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-        // neighbouring threads read neighbouring elements
-        const int ca = kKind == kForward ? i % kDepth : i / kTile, fa = kKind == kForward ? i / kDepth : i % kTile;
-        float v = 0.f;
-        if (f0 + fa < p.m && c0 + ca < depth) {
-          const int64_t at = kKind == kForward     ? group * p.a_group + (f0 + fa) * p.a_pitch + c0 + ca
-                             : kKind == kInputGrad ? group * p.a_group + (c0 + ca) * p.a_pitch + f0 + fa
-                                                   : int64_t(begin + c0 + ca) * p.a_pitch + f0 + fa;
-          v = load_h16(p.a, at, fp16);
-        }
-        sa[ca][fa] = v;
-        const int cb = kKind == kWeightGrad ? i / kTile : i % kDepth, jb = kKind == kWeightGrad ? i % kTile : i / kDepth;
-        v = 0.f;
-        if (j0 + jb < count && c0 + cb < depth) {
-          const int64_t at = kKind == kWeightGrad ? int64_t(begin + c0 + cb) * p.b_pitch + j0 + jb
-                                                  : int64_t(begin + j0 + jb) * p.b_pitch + c0 + cb;
-          v = load_h16(p.b, at, fp16);
-        }
-        sb[cb][jb] = v;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int c = 0; c < kDepth; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[c][tx + 16 * i], sb[c][ty + 16 * j], acc[i][j]);
-      __syncthreads();
-    }
-    for (int j = 0; j < 4; ++j)
-      for (int i = 0; i < 4; ++i) {
-        const int row = j0 + ty + 16 * j, f = f0 + tx + 16 * i;
-        if (row >= count || f >= p.m) continue;
-        const int64_t at = kKind == kWeightGrad ? int64_t(group) * p.n + row : int64_t(begin) + row;
-        finish_element(p.epi, p.m, at, f, acc[i][j]);
-      }
+__device__ __forceinline__ Tile locate(int tile, const ProductArgs& p, const TileShape& s, const SmemTail* t) {
+  Tile r;
+  r.split = 0;
+  if (s.splits > 1) {
+    r.split = tile % s.splits;
+    tile /= s.splits;
   }
+  int blocks, local;
+  if (kKind == kWeightGrad) {
+    blocks = s.row_blocks;
+    const int per_group = blocks * s.f_tiles;
+    r.group = p.groups == 1 ? 0 : tile / per_group;
+    local = tile - r.group * per_group;
+  } else {
+    // the last group whose first tile is not past `tile`: 32 coarse probes, then one per group
+    int lo = 0;
+    if (p.groups > 1) {
+      const int lane = threadIdx.x & 31;
+      const int step = (p.groups + 31) / 32;
+      const int coarse = lane * step;
+      lo = (__popc(__ballot_sync(0xffffffffu, coarse < p.groups && t->blocks[coarse] * s.f_tiles <= tile)) - 1) * step;
+      const int fine = lo + lane;
+      lo += __popc(__ballot_sync(0xffffffffu, lane < step && fine < p.groups && t->blocks[fine] * s.f_tiles <= tile)) - 1;
+    }
+    r.group = lo;
+    blocks = t->blocks[lo + 1] - t->blocks[lo];
+    local = tile - t->blocks[lo] * s.f_tiles;
+  }
+  int band = local / (kBand * s.f_tiles);
+  local -= band * kBand * s.f_tiles;
+  const int in_band = min(kBand, blocks - band * kBand);
+  const int f = local / in_band;
+  const int j = band * kBand + local - f * in_band;
+  r.f0 = f * kTileFeatures;
+  if (kKind == kWeightGrad) {
+    int begin, end;
+    segment_of(p, r.group, begin, end);
+    r.b_row = j * kTileRows;
+    const int left = p.n - r.b_row;
+    r.cols = left > 128 ? 256 : 128;  // whole 64-column boxes in each CTA
+    r.valid = min(left, r.cols);
+    r.out_row = int64_t(r.group) * p.n + r.b_row;
+    r.c_begin = begin;
+    r.depth = end - begin;
+  } else {
+    const int len = t->len[r.group];
+    const int per = ((len + blocks - 1) / blocks + 31) / 32 * 32;  // balanced parts
+    const int start = j * per;
+    r.b_row = t->begin[r.group] + start;
+    r.valid = max(min(per, len - start), 0);
+    r.cols = max((r.valid + 31) / 32 * 32, 32);
+    r.out_row = r.b_row;
+    r.c_begin = 0;
+    r.depth = p.k;
+  }
+  const int steps = (r.depth + kStep - 1) / kStep;
+  r.step0 = s.splits > 1 ? int(int64_t(steps) * r.split / s.splits) : 0;
+  r.step1 = s.splits > 1 ? int(int64_t(steps) * (r.split + 1) / s.splits) : steps;
+  return r;
+}
+
+// kFinish: the output is more than the rounded sum (bias, activation, residual or slope)
+template <int kKind, bool kFinish>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const TileShape shape) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+  const uint32_t ring = raw_addr + pad;
+  SmemTail* t = reinterpret_cast<SmemTail*>(smem_raw + pad + kRingBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int worker = blockIdx.x >> 1, workers = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&maps.a);
+    for (int s = 0; s < kMaxStages; ++s) {
+      mbar_init(smem_u32(&t->full[s]), kKind == kWeightGrad ? 2 : 1);
+      mbar_init(smem_u32(&t->empty[s]), 1);
+      mbar_init(smem_u32(&t->raw[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&t->acc_full[b]), 1);
+      mbar_init(smem_u32(&t->acc_empty[b]), 2 * kEpilogueWarps);
+    }
+    t->abort_flag = 0;
+    t->max_len = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 3) tmem_alloc_pair(smem_u32(&t->tmem_base), kTmemCols);
+  __syncthreads();
+
+  int total_tiles;
+  int half_rows = 128;  // rows of b that a CTA loads for a step at most
+  if (kKind == kWeightGrad) {
+    total_tiles = p.groups * shape.row_blocks * shape.f_tiles;
+    if (p.n <= 128) half_rows = 64;
+  } else {
+    int longest = 0;
+    for (int g = threadIdx.x; g < p.groups; g += kThreads) {
+      int begin, end;
+      segment_of(p, g, begin, end);
+      t->begin[g] = begin;
+      t->len[g] = end - begin;
+      longest = max(longest, end - begin);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0 && longest > 0) atomicMax(&t->max_len, longest);
+    __syncthreads();
+    if (warp == 0) {  // row blocks before each group: every lane adds up a run of groups
+      const int per = (p.groups + 31) / 32;
+      const int lo = min(lane * per, p.groups), hi = min(lo + per, p.groups);
+      int sum = 0;
+      for (int g = lo; g < hi; ++g) sum += (t->len[g] + kTileRows - 1) / kTileRows;
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      int run = incl - sum;
+      for (int g = lo; g < hi; ++g) {
+        t->blocks[g] = run;
+        run += (t->len[g] + kTileRows - 1) / kTileRows;
+      }
+      if (lane == 31) t->blocks[p.groups] = incl;
+    }
+    __syncthreads();
+    total_tiles = t->blocks[p.groups] * shape.f_tiles;
+    half_rows = min(128, (t->max_len + 31) / 32 * 16);
+  }
+  total_tiles *= shape.splits;
+  const int stage_bytes = kABytes + max(half_rows, 16) * 128;
+  const int stages = min(kMaxStages, int(kRingBytes) / stage_bytes);
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers exist
+  tc_fence_after();
+  const uint32_t tmem = t->tmem_base;
+  WaitCtx ctx{&t->abort_flag, g_status, wait_limit_ns(g_status)};
+
+  if (warp == 0) {
+    // ---------------- loads ----------------
+    if (lane < kBoxes) prefetch_tmap(&maps.b[lane]);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = worker; ok && tile < total_tiles; tile += workers) {
+      const Tile c = locate<kKind>(tile, p, shape, t);
+      const int half = c.cols >> 1;
+      const int f = c.f0 + int(rank) * 128, j = c.b_row + int(rank) * half;
+      const uint32_t bytes = kABytes + half * 128;
+      const bool ragged = kKind == kWeightGrad && c.depth % kStep != 0;
+      for (int kb = c.step0; kb < c.step1; ++kb) {
+        ok = mbar_wait(smem_u32(&t->empty[stage]), phase ^ 1, ctx, 21);
+        if (!ok) break;
+        if (elect_one()) {
+          const bool tail = ragged && kb == c.depth / kStep;
+          const uint32_t own_bar = smem_u32(tail ? &t->raw[stage] : &t->full[stage]);
+          const uint32_t bar = tail ? map_to_cta(own_bar, rank) : map_to_cta(own_bar, 0);
+          if (tail) {
+            mbar_expect_tx(own_bar, bytes);
+          } else if (rank == 0) {
+            mbar_expect_tx(own_bar, 2 * bytes);
+            if (kKind == kWeightGrad) mbar_arrive(own_bar);
+          }
+          const uint32_t a_dst = ring + stage * stage_bytes, b_dst = a_dst + kABytes;
+          const int k0 = kb * kStep;
+          if (kKind == kForward) {
+            tma_load_3d_pair(a_dst, &maps.a, k0, f, c.group, bar);
+          } else if (kKind == kInputGrad) {
+            tma_load_3d_pair(a_dst, &maps.a, f, k0, c.group, bar);
+            tma_load_3d_pair(a_dst + 8192, &maps.a, f + 64, k0, c.group, bar);
+          } else {
+            tma_load_3d_pair(a_dst, &maps.a, f, c.c_begin + k0, 0, bar);
+            tma_load_3d_pair(a_dst + 8192, &maps.a, f + 64, c.c_begin + k0, 0, bar);
+          }
+          if (kKind == kWeightGrad) {
+            tma_load_3d_pair(b_dst, &maps.b[2], j, c.c_begin + k0, 0, bar);
+            if (half == 128) tma_load_3d_pair(b_dst + 8192, &maps.b[2], j + 64, c.c_begin + k0, 0, bar);
+          } else {
+            int r = 0;
+#pragma unroll
+            for (int b = kBoxes - 1; b >= 0; --b)
+              if (half & (16 << b)) {
+                tma_load_3d_pair(b_dst + r * 128, &maps.b[b], k0, j + r, 0, bar);
+                r += 16 << b;
+              }
+          }
+        }
+        __syncwarp();
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- products (the pair's first CTA) ----------------
+    int stage = 0;
+    uint32_t phase = 0, it = 0;
+    bool ok = true;
+    const uint32_t fmt = p.epi.fp16 ? 0u : 1u;
+    for (int tile = worker; rank == 0 && ok && tile < total_tiles; tile += workers, ++it) {
+      const Tile c = locate<kKind>(tile, p, shape, t);
+      const uint32_t buf = it & 1, use = it >> 1;
+      ok = mbar_wait_cluster(smem_u32(&t->acc_empty[buf]), (use & 1) ^ 1, ctx, 22);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t d = tmem + buf * 256;
+      const uint32_t idesc = make_idesc(fmt, fmt, 256, uint32_t(c.cols)) | (kKind != kForward ? 1u << 15 : 0u) |
+                             (kKind == kWeightGrad ? 1u << 16 : 0u);
+      for (int kb = c.step0; kb < c.step1; ++kb) {
+        ok = mbar_wait_cluster(smem_u32(&t->full[stage]), phase, ctx, 23);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t a_addr = ring + stage * stage_bytes;
+          const uint64_t a_desc = kKind == kForward ? make_kmajor_sw128_desc(a_addr) : make_mnmajor_sw128_desc(a_addr);
+          const uint64_t b_desc = kKind == kWeightGrad ? make_mnmajor_sw128_desc(a_addr + kABytes)
+                                                       : make_kmajor_sw128_desc(a_addr + kABytes);
+          constexpr int kAStep = kKind == kForward ? 2 : 128, kBStep = kKind == kWeightGrad ? 128 : 2;
+          const int parts = min(4, (c.depth - kb * kStep + 15) / 16);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < parts)
+              umma_h16_pair(d, a_desc + kAStep * k, b_desc + kBStep * k, idesc, kb > c.step0 || k > 0);
+          tc_commit_pair(smem_u32(&t->empty[stage]));
+        }
+        __syncwarp();
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+      }
+      if (ok && elect_one()) tc_commit_pair(smem_u32(&t->acc_full[buf]));
+      __syncwarp();
+    }
+  } else if (warp == 2) {
+    // ---------------- weight gradient: rows past the segment's end become zeros ----------------
+    int stage = 0;
+    uint32_t phases = 0;  // parity of raw[stage], one bit each
+    bool ok = true;
+    for (int tile = worker; kKind == kWeightGrad && ok && tile < total_tiles; tile += workers) {
+      const Tile c = locate<kKind>(tile, p, shape, t);
+      const int last = c.depth / kStep;
+      if (c.depth % kStep != 0 && last >= c.step0 && last < c.step1) {
+        const int at = (stage + last - c.step0) % stages;
+        ok = mbar_wait(smem_u32(&t->raw[at]), (phases >> at) & 1, ctx, 24);
+        if (!ok) break;
+        phases ^= 1u << at;
+        // a row is 128 bytes of each 64-element box; the products read whole groups of 16 rows
+        const int from = c.depth - last * kStep, to = (from + 15) / 16 * 16;
+        const int boxes = 2 + (c.cols >> 7);
+        const uint32_t base = ring + at * stage_bytes;
+        for (int i = lane; i < boxes * (to - from) * 8; i += 32) {
+          const int box = i / ((to - from) * 8), rest = i - box * (to - from) * 8;
+          const uint32_t addr = base + box * 8192 + (from + rest / 8) * 128 + (rest & 7) * 16;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
+        }
+        fence_proxy_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&t->full[at]), 0));
+        __syncwarp();
+      }
+      stage = (stage + c.step1 - c.step0) % stages;
+    }
+  } else if (warp >= kFirstEpilogueWarp) {
+    // ---------------- epilogue: each warp on 32 features ----------------
+    const int quarter = warp & 3;                                   // tensor-memory lanes 32*quarter .. +31
+    const int first_chunk = (warp - kFirstEpilogueWarp) >> 2;       // chunks of 16 output rows, every other one
+    float* turn = t->turn[warp - kFirstEpilogueWarp];
+    uint32_t it = 0;
+    for (int tile = worker; tile < total_tiles; tile += workers, ++it) {
+      const Tile c = locate<kKind>(tile, p, shape, t);
+      const uint32_t buf = it & 1, use = it >> 1;
+      const int f = c.f0 + int(rank) * 128 + quarter * 32 + 4 * (lane & 7);
+      Bias4 bias{};
+      if (kFinish && shape.splits == 1) bias = load_bias4(p.epi, p.m, f);
+      if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
+      tc_fence_after();
+      const bool summed = c.step1 > c.step0;
+      const uint32_t lanes = tmem + buf * 256 + (uint32_t(quarter * 32) << 16);
+      const int chunks = (c.valid + 15) >> 4;
+      auto emit = [&](int chunk, const uint32_t (&v)[16]) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) turn[i * 32 + lane] = summed ? __uint_as_float(v[i]) : 0.f;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = chunk * 16 + (lane >> 3) + 4 * i;
+          const float4 s = *reinterpret_cast<const float4*>(turn + ((lane >> 3) + 4 * i) * 32 + 4 * (lane & 7));
+          if (row < c.valid && f < p.m) {
+            float z[4] = {s.x, s.y, s.z, s.w};
+            if (shape.splits > 1) {
+              const int64_t at = (c.split * shape.partial_rows + c.out_row + row) * shape.partial_pitch + f;
+              *reinterpret_cast<float4*>(shape.partial + at) = s;
+            } else if (kFinish) {
+              finish4(p.epi, p.m, c.out_row + row, f, z, bias, shape.vec);
+            } else if (shape.vec) {
+              const int64_t at = (c.out_row + row) * p.m + f;
+              if (p.epi.out_fp32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.epi.out) + at) = s;
+              else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.epi.out) + at) = pack_h16x4(z, p.epi.fp16);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (f + e < p.m) {
+                  const int64_t at = (c.out_row + row) * p.m + f + e;
+                  if (p.epi.out_fp32) reinterpret_cast<float*>(p.epi.out)[at] = z[e];
+                  else reinterpret_cast<uint16_t*>(p.epi.out)[at] = to_h16(z[e], p.epi.fp16);
+                }
+            }
+          }
+        }
+        __syncwarp();
+      };
+      bool released = false;
+      auto release = [&]() {  // this warp's share is in registers: the accumulator may be overwritten
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&t->acc_empty[buf]), 0));
+        released = true;
+      };
+      for (int k = first_chunk; k < chunks; k += 4) {
+        uint32_t va[16], vb[16];
+        const bool two = k + 2 < chunks;
+        tmem_ld16(lanes + k * 16, va);
+        if (two) tmem_ld16(lanes + (k + 2) * 16, vb);
+        tmem_ld_wait();
+        if (k + 4 >= chunks) release();
+        emit(k, va);
+        if (two) emit(k + 2, vb);
+      }
+      if (!released) release();
+    }
+  }
+
+  // ---------------- teardown ----------------
+  __syncwarp();
+  tc_fence_before();
+  if (t->abort_flag) {
+    // a wait was abandoned: copies and products still in flight get time to land
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);
+  }
+  cluster_sync();  // the other CTA arrives on this one's barriers no more
+  tc_fence_after();
+  if (warp == 3) tmem_dealloc_pair(tmem, kTmemCols);
+}
+
+// Split sums: the parts added in order, then the epilogue.
+__global__ void __launch_bounds__(256) join_kernel(const ProductArgs p, const TileShape s) {
+  const int64_t vecs = s.partial_pitch / 4, total = s.partial_rows * vecs;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+    const int64_t row = i / vecs;
+    const int f = int(i - row * vecs) * 4;
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* part = s.partial + row * s.partial_pitch + f;
+    for (int k = 0; k < s.splits; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(part + k * s.partial_rows * s.partial_pitch);
+      z[0] += v.x;
+      z[1] += v.y;
+      z[2] += v.z;
+      z[3] += v.w;
+    }
+    finish4(p.epi, p.m, row, f, z, load_bias4(p.epi, p.m, f), s.vec);
+  }
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// A dense product of few tiles leaves most pairs idle: its sums are split, at least four steps to a part.
+int split_count(ProductKind kind, int64_t rows, int m, int n, int k, int device) {
+  const int pairs = device_sm_count(device) / 2;
+  const int64_t tiles = ceil_div(m, kTileFeatures) * ceil_div(kind == kWeightGrad ? n : rows, kTileRows);
+  const int64_t steps = ceil_div(kind == kWeightGrad ? rows : k, kStep);
+  int64_t s = tiles > 0 ? pairs / tiles : 1;
+  if (s > steps / 4) s = steps / 4;
+  return int(s < 1 ? 1 : s);
+}
+int64_t partial_pitch(int m) { return ceil_div(m, 4) * 4; }
+
+// Tiled view of 16-bit elements: c0 side by side, c1 `pitch` elements apart, c2 `group` elements apart.
+int make_map(CUtensorMap* map, const void* base, int64_t c0, int64_t c1, int64_t c2, int64_t pitch, int64_t group,
+             uint32_t box1, int fp16) {
+  return make_tensor_map_3d(map, base, uint64_t(c0), uint64_t(c1), uint64_t(c2), uint64_t(pitch) * 2,
+                            uint64_t(group) * 2, box1, fp16);
+}
+
+bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+using KernelFn = void (*)(const Maps, const ProductArgs, const TileShape);
+template <int kKind>
+KernelFn kernel_of(bool finish) {
+  if (kKind == kForward && finish) return product_kernel<kForward, true>;
+  return product_kernel<kKind, false>;
 }
 
 }  // namespace
 
-int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaStream_t stream) {
-  (void)device;
-  const int64_t most = kind == kWeightGrad ? args.n : args.rows;
-  const unsigned by = unsigned(most <= 0 ? 1 : (most + kTile - 1) / kTile < 512 ? (most + kTile - 1) / kTile : 512);
-  const dim3 grid((args.m + kTile - 1) / kTile, by, args.groups);
-  if (kind == kForward) product_kernel<kForward><<<grid, 256, 0, stream>>>(args);
-  else if (kind == kInputGrad) product_kernel<kInputGrad><<<grid, 256, 0, stream>>>(args);
-  else product_kernel<kWeightGrad><<<grid, 256, 0, stream>>>(args);
+int64_t product_workspace_bytes(ProductKind kind, int rows, int m, int n, int k, int device) {
+  const int s = split_count(kind, rows, m, n, k, device);
+  return s > 1 ? s * int64_t(kind == kWeightGrad ? n : rows) * partial_pitch(m) * 4 : 0;
+}
+
+int product_status(int* status_out, int clear, cudaStream_t stream) {
+  MB200_CHECK_CUDA(cudaStreamSynchronize(stream));
+  MB200_CHECK_CUDA(cudaMemcpyFromSymbol(status_out, g_status, sizeof(int)));
+  const int zero = 0;
+  if (clear) MB200_CHECK_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(int)));
+  return kOk;
+}
+
+int launch_product(ProductKind kind, const ProductArgs& args, void* workspace, int64_t workspace_bytes, int device,
+                   cudaStream_t stream) {
+  const int sms = device_sm_count(device);
+  MB200_REQUIRE(sms > 1, kCudaError, "product: cannot read the SM count of device %d", device);
+  const bool weight = kind == kWeightGrad;
+  TileShape s{};
+  s.f_tiles = int(ceil_div(args.m, kTileFeatures));
+  s.row_blocks = weight ? int(ceil_div(args.n, kTileRows)) : 0;
+  s.splits = args.offsets ? 1 : split_count(kind, args.rows, args.m, args.n, args.k, device);
+  s.partial_rows = weight ? args.n : args.rows;
+  s.partial_pitch = partial_pitch(args.m);
+  if (s.splits > 1) {
+    const int64_t need = s.splits * s.partial_rows * s.partial_pitch * 4;
+    MB200_REQUIRE(workspace && aligned_to(workspace, 16), kInvalidArgument, "product: needs a 16-byte aligned workspace");
+    MB200_REQUIRE(workspace_bytes >= need, kWorkspaceTooSmall, "product: workspace %lld < %lld bytes",
+                  (long long)workspace_bytes, (long long)need);
+    s.partial = reinterpret_cast<float*>(workspace);
+  }
+  const int64_t tiles = (weight ? int64_t(args.groups) * s.row_blocks : int64_t(args.rows) / kTileRows + args.groups) *
+                        s.f_tiles * s.splits;
+  MB200_REQUIRE(tiles < (int64_t(1) << 30), kUnsupportedShape, "product: %lld tiles do not fit 32-bit tile numbers",
+                (long long)tiles);
+  const Epilogue& e = args.epi;
+  s.vec = args.m % 4 == 0 && aligned_to(e.out, e.out_fp32 ? 16 : 8) && (!e.slope || aligned_to(e.slope, 8)) &&
+          (!e.residual || (aligned_to(e.residual, 8) && e.residual_pitch % 4 == 0));
+
+  Maps maps;
+  int rc;
+  const int fp16 = e.fp16;
+  if (kind == kForward) rc = make_map(&maps.a, args.a, args.k, args.m, args.groups, args.a_pitch, args.a_group, 128, fp16);
+  else if (kind == kInputGrad) rc = make_map(&maps.a, args.a, args.m, args.k, args.groups, args.a_pitch, args.a_group, 64, fp16);
+  else rc = make_map(&maps.a, args.a, args.m, args.rows, 1, args.a_pitch, 0, 64, fp16);
+  if (rc) return rc;
+  for (int i = 0; i < kBoxes; ++i)
+    if ((rc = make_map(&maps.b[i], args.b, weight ? args.n : args.k, args.rows, 1, args.b_pitch, 0, 16u << i, fp16))) return rc;
+
+  const bool finish = e.bias || e.act || e.residual || e.slope;
+  const int variant = kind == kForward ? (finish ? 1 : 0) : kind == kInputGrad ? 2 : 3;
+  const KernelFn kernel = kind == kForward     ? kernel_of<kForward>(finish)
+                          : kind == kInputGrad ? kernel_of<kInputGrad>(false)
+                                               : kernel_of<kWeightGrad>(false);
+  static std::atomic<bool> configured[kMaxDevices][4];
+  if (device < 0 || device >= kMaxDevices || !configured[device][variant].load(std::memory_order_acquire)) {
+    MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)));
+    if (device >= 0 && device < kMaxDevices) configured[device][variant].store(true, std::memory_order_release);
+  }
+  const int64_t pairs = tiles < sms / 2 ? (tiles < 1 ? 1 : tiles) : sms / 2;
+  kernel<<<unsigned(2 * pairs), kThreads, kSmemBytes, stream>>>(maps, args, s);
   MB200_CHECK_CUDA(cudaGetLastError());
+  if (s.splits > 1) {
+    const int64_t blocks = ceil_div(s.partial_rows * s.partial_pitch / 4, 256);
+    join_kernel<<<unsigned(blocks < 8 * sms ? blocks : 8 * sms), 256, 0, stream>>>(args, s);
+    MB200_CHECK_CUDA(cudaGetLastError());
+  }
   return kOk;
 }
 
