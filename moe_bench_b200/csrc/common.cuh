@@ -454,6 +454,11 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same without that order, for what the tensor cores' own fences order: a release waits for the thread's
+// earlier global stores.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // mbar_wait for a barrier that the other CTA's threads arrive on.
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, WaitCtx& ctx, int where) {
   uint32_t spins = 0;

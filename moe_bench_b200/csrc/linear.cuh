@@ -56,40 +56,55 @@ __device__ __forceinline__ float load_h16(const void* p, int64_t i, int fp16) {
               : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
 }
 
-// act(z), and with kSlope act'(z).  Both stay finite wherever z is; NaN stays NaN in act(z).
-template <bool kSlope>
-__device__ __forceinline__ float activate(int act, float z, float& slope) {
-  slope = 1.f;
+// 1 / (1 + exp(-v)): exp and the quotient are good to about 2^-22 of their values plus |v| 2^-24, far inside any 16-bit
+// rounding and about 2 units of an fp32 output.
+__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+
+// act(z) in place, and with kSlope act'(z), for values that have nothing to do with one another.  Both stay finite
+// wherever z is; NaN stays NaN in act(z).
+template <bool kSlope, int kCount>
+__device__ __forceinline__ void activate(int act, float (&z)[kCount], float (&slope)[kCount]) {
   switch (act) {
     case kActRelu:
-      if (kSlope) slope = z > 0.f ? 1.f : 0.f;
-      return z < 0.f ? 0.f : z;
-    case kActSilu: {
-      const float s = 1.f / (1.f + expf(-z));
-      if (kSlope) slope = s * (1.f + z * (1.f - s));
-      return z * s;
-    }
-    case kActGelu: {
-      const float c = 0.5f + 0.5f * erff(z * 0.70710678118654752f);
-      // below -3 the sum of 1/2 and erf/2 cancels: the same value by the complement
-      const float cdf = z < -1.f ? 0.5f * erfcf(-z * 0.70710678118654752f) : c;
-      if (kSlope) slope = cdf + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-      return z * cdf;
-    }
-    case kActGeluTanh: {
-      // (1 + tanh u) / 2 = 1 / (1 + exp(-2u)); past |z| = 30 it is 0 or 1 in fp32, and z^3 stays finite
-      const float t = fminf(fmaxf(z, -30.f), 30.f);
-      const float u = 0.79788456080286536f * (t + 0.044715f * t * t * t);
-      const float c = 1.f / (1.f + expf(-2.f * u));
-      if (kSlope) slope = c + 2.f * t * c * (1.f - c) * (0.79788456080286536f * (1.f + 0.134145f * t * t));
-      return z * c;
-    }
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) {
+        if (kSlope) slope[i] = z[i] > 0.f ? 1.f : 0.f;
+        z[i] = z[i] < 0.f ? 0.f : z[i];
+      }
+      break;
+    case kActSilu:
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) {
+        const float s = sigmoid(z[i]);
+        if (kSlope) slope[i] = s * (1.f + z[i] * (1.f - s));
+        z[i] *= s;
+      }
+      break;
+    case kActGelu:
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) {
+        // (1 + erf(z / sqrt 2)) / 2 by the complement: the sum cancels below 0
+        const float c = 0.5f * erfcf(-z[i] * 0.70710678118654752f);
+        if (kSlope) slope[i] = c + z[i] * (__expf(-0.5f * z[i] * z[i]) * 0.39894228040143268f);
+        z[i] *= c;
+      }
+      break;
+    case kActGeluTanh:
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) {
+        // (1 + tanh u) / 2 = sigmoid(2u); past |z| = 30 it is 0 or 1 in fp32, and z^3 stays finite
+        const float t = fminf(fmaxf(z[i], -30.f), 30.f);
+        const float c = sigmoid(1.5957691216057307f * (t + 0.044715f * t * t * t));
+        if (kSlope) slope[i] = c + t * c * (1.f - c) * (1.5957691216057307f * (1.f + 0.134145f * t * t));
+        z[i] *= c;
+      }
+      break;
     default:
-      return z;
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) slope[i] = 1.f;
   }
 }
 
-// `residual` may be `out`: no promise that it is constant.
 struct Bias4 {
   float v[4];
 };
@@ -101,57 +116,75 @@ __device__ __forceinline__ Bias4 load_bias4(const Epilogue& e, int m, int f) {
       if (f + i < m) b.v[i] = e.bias_fp32 ? __ldg(reinterpret_cast<const float*>(e.bias) + f + i) : load_h16(e.bias, f + i, e.fp16);
   return b;
 }
-__device__ __forceinline__ uint2 pack_h16x4(const float (&v)[4], int fp16) {
-  return make_uint2(pack_h16x2(v[0], v[1], fp16), pack_h16x2(v[2], v[3], fp16));
-}
-
-// One element.
-__device__ __forceinline__ void finish_element(const Epilogue& e, int m, int64_t row, int f, float z) {
-  if (e.bias) z += e.bias_fp32 ? reinterpret_cast<const float*>(e.bias)[f] : load_h16(e.bias, f, e.fp16);
-  float slope = 1.f;
-  float y;
-  if (e.slope) {
-    y = activate<true>(e.act, z, slope);
-    reinterpret_cast<uint16_t*>(e.slope)[row * m + f] = to_h16(slope, e.fp16);
-  } else {
-    y = activate<false>(e.act, z, slope);
-  }
-  if (e.residual) y += load_h16(e.residual, row * e.residual_pitch + f, e.fp16);
-  if (e.out_fp32)
-    reinterpret_cast<float*>(e.out)[row * m + f] = y;
-  else
-    reinterpret_cast<uint16_t*>(e.out)[row * m + f] = to_h16(y, e.fp16);
-}
-
-// Four features side by side, f a multiple of 4.  `vec`: every tensor takes them as one access (then m is a multiple of 4).
-__device__ __forceinline__ void finish4(const Epilogue& e, int m, int64_t row, int f, float (&z)[4], const Bias4& bias,
-                                        bool vec) {
-  if (!vec) {
+// kRows output rows, `step` apart, x four features side by side; rows from `last` on and features from m on do not exist.
+// `vec`: every tensor takes four features as one access (then m is a multiple of 4).
+// The residual may be the output's buffer: its loads promise nothing, and come before the rows' stores.
+template <int kRows>
+struct Residual4 {
+  uint2 v[kRows];
+};
+template <int kRows>
+__device__ __forceinline__ Residual4<kRows> load_residual4(const Epilogue& e, int m, int64_t row, int step, int64_t last, int f, bool vec) {
+  Residual4<kRows> r{};
+  if (e.residual) {
+    const uint16_t* at = reinterpret_cast<const uint16_t*>(e.residual) + f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (f + i < m) finish_element(e, m, row, f + i, z[i]);
+    for (int i = 0; i < kRows; ++i)
+      if (row + i * step < last) {
+        const uint16_t* p = at + (row + i * step) * e.residual_pitch;
+        if (vec) {
+          if (f < m) r.v[i] = *reinterpret_cast<const uint2*>(p);
+        } else {
+          uint16_t h[4] = {};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (f + k < m) h[k] = p[k];
+          r.v[i] = make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
+        }
+      }
+  }
+  return r;
+}
+
+__device__ __forceinline__ void store4(void* out, int fp32, int fp16, int m, int64_t row, int f, const float* v, bool vec) {
+  if (f >= m) return;
+  const int64_t at = row * m + f;
+  if (vec) {
+    if (fp32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + at) =
+        make_uint2(pack_h16x2(v[0], v[1], fp16), pack_h16x2(v[2], v[3], fp16));
     return;
   }
-  float slope[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) z[i] += bias.v[i];
+  for (int k = 0; k < 4; ++k)
+    if (f + k < m) {
+      if (fp32) reinterpret_cast<float*>(out)[at + k] = v[k];
+      else reinterpret_cast<uint16_t*>(out)[at + k] = to_h16(v[k], fp16);
+    }
+}
+
+template <int kRows>
+__device__ __forceinline__ void finish4(const Epilogue& e, int m, int64_t row, int step, int64_t last, int f, float (&z)[4 * kRows],
+                                        const Bias4& bias, const Residual4<kRows>& res, bool vec) {
+  float slope[4 * kRows];
+#pragma unroll
+  for (int i = 0; i < 4 * kRows; ++i) z[i] += bias.v[i & 3];
   if (e.slope) {
+    activate<true>(e.act, z, slope);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = activate<true>(e.act, z[i], slope[i]);
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(e.slope) + row * m + f) = pack_h16x4(slope, e.fp16);
+    for (int i = 0; i < kRows; ++i)
+      if (row + i * step < last) store4(e.slope, 0, e.fp16, m, row + i * step, f, slope + 4 * i, vec);
   } else if (e.act) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = activate<false>(e.act, z[i], slope[i]);
+    activate<false>(e.act, z, slope);
   }
-  if (e.residual) {
-    const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(e.residual) + row * e.residual_pitch + f);
+  if (e.residual)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] += load_h16(&r, i, e.fp16);
-  }
-  if (e.out_fp32)
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(e.out) + row * m + f) = make_float4(z[0], z[1], z[2], z[3]);
-  else
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(e.out) + row * m + f) = pack_h16x4(z, e.fp16);
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[4 * i + k] += load_h16(&res.v[i], k, e.fp16);
+#pragma unroll
+  for (int i = 0; i < kRows; ++i)
+    if (row + i * step < last) store4(e.out, e.out_fp32, e.fp16, m, row + i * step, f, z + 4 * i, vec);
 }
 
 // products.cu

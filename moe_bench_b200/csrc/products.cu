@@ -365,54 +365,59 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
       const bool summed = c.step1 > c.step0;
       const uint32_t lanes = tmem + buf * 256 + (uint32_t(quarter * 32) << 16);
       const int chunks = (c.valid + 15) >> 4;
-      auto emit = [&](int chunk, const uint32_t (&v)[16]) {
+      const int64_t last = c.out_row + c.valid;
+      auto emit = [&](int chunk, const uint32_t (&v)[16], const Residual4<4>& res) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) turn[i * 32 + lane] = summed ? __uint_as_float(v[i]) : 0.f;
         __syncwarp();
+        float z[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int row = chunk * 16 + (lane >> 3) + 4 * i;
           const float4 s = *reinterpret_cast<const float4*>(turn + ((lane >> 3) + 4 * i) * 32 + 4 * (lane & 7));
-          if (row < c.valid && f < p.m) {
-            float z[4] = {s.x, s.y, s.z, s.w};
-            if (shape.splits > 1) {
-              const int64_t at = (c.split * shape.partial_rows + c.out_row + row) * shape.partial_pitch + f;
-              *reinterpret_cast<float4*>(shape.partial + at) = s;
-            } else if (kFinish) {
-              finish4(p.epi, p.m, c.out_row + row, f, z, bias, shape.vec);
-            } else if (shape.vec) {
-              const int64_t at = (c.out_row + row) * p.m + f;
-              if (p.epi.out_fp32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.epi.out) + at) = s;
-              else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.epi.out) + at) = pack_h16x4(z, p.epi.fp16);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (f + e < p.m) {
-                  const int64_t at = (c.out_row + row) * p.m + f + e;
-                  if (p.epi.out_fp32) reinterpret_cast<float*>(p.epi.out)[at] = z[e];
-                  else reinterpret_cast<uint16_t*>(p.epi.out)[at] = to_h16(z[e], p.epi.fp16);
-                }
-            }
-          }
+          z[4 * i] = s.x;
+          z[4 * i + 1] = s.y;
+          z[4 * i + 2] = s.z;
+          z[4 * i + 3] = s.w;
         }
         __syncwarp();
+        const int64_t row = c.out_row + chunk * 16 + (lane >> 3);
+        if (shape.splits > 1) {
+          if (f < p.m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (row + 4 * i < last)
+                *reinterpret_cast<float4*>(shape.partial + (c.split * shape.partial_rows + row + 4 * i) * shape.partial_pitch + f) =
+                    make_float4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
+        } else if (kFinish) {
+          finish4<4>(p.epi, p.m, row, 4, last, f, z, bias, res, shape.vec);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (row + 4 * i < last) store4(p.epi.out, p.epi.out_fp32, p.epi.fp16, p.m, row + 4 * i, f, z + 4 * i, shape.vec);
+        }
       };
       bool released = false;
       auto release = [&]() {  // this warp's share is in registers: the accumulator may be overwritten
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&t->acc_empty[buf]), 0));
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&t->acc_empty[buf]), 0));
         released = true;
       };
       for (int k = first_chunk; k < chunks; k += 4) {
         uint32_t va[16], vb[16];
         const bool two = k + 2 < chunks;
+        Residual4<4> ra{}, rb{};
+        if (kFinish && shape.splits == 1) {
+          const int64_t row = c.out_row + k * 16 + (lane >> 3);
+          ra = load_residual4<4>(p.epi, p.m, row, 4, last, f, shape.vec);
+          if (two) rb = load_residual4<4>(p.epi, p.m, row + 32, 4, last, f, shape.vec);
+        }
         tmem_ld16(lanes + k * 16, va);
         if (two) tmem_ld16(lanes + (k + 2) * 16, vb);
         tmem_ld_wait();
         if (k + 4 >= chunks) release();
-        emit(k, va);
-        if (two) emit(k + 2, vb);
+        emit(k, va, ra);
+        if (two) emit(k + 2, vb, rb);
       }
       if (!released) release();
     }
@@ -445,7 +450,8 @@ __global__ void __launch_bounds__(256) join_kernel(const ProductArgs p, const Ti
       z[2] += v.z;
       z[3] += v.w;
     }
-    finish4(p.epi, p.m, row, f, z, load_bias4(p.epi, p.m, f), s.vec);
+    finish4<1>(p.epi, p.m, row, 1, row + 1, f, z, load_bias4(p.epi, p.m, f),
+               load_residual4<1>(p.epi, p.m, row, 1, row + 1, f, s.vec), s.vec);
   }
 }
 
