@@ -71,6 +71,7 @@ struct TileShape {
   float* partial;   // [splits][output rows][partial_pitch] where splits > 1
   int64_t partial_rows, partial_pitch;
   int vec;          // the epilogue may access four features at once
+  int vec8;         // nothing but sums rounded to 16 bits, eight features at once
 };
 
 // first failure of a wait, wait limit in ms, 0, 0
@@ -335,12 +336,12 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
         // a row is 128 bytes of each 64-element box; the products read whole groups of 16 rows
         const int from = c.depth - last * kStep, to = (from + 15) / 16 * 16;
         const int boxes = 2 + (c.cols >> 7);
-        const uint32_t base = ring + at * stage_bytes;
-        for (int i = lane; i < boxes * (to - from) * 8; i += 32) {
-          const int box = i / ((to - from) * 8), rest = i - box * (to - from) * 8;
-          const uint32_t addr = base + box * 8192 + (from + rest / 8) * 128 + (rest & 7) * 16;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
-        }
+        const uint32_t base = ring + at * stage_bytes + (lane & 7) * 16;
+        for (int r = from + (lane >> 3); r < to; r += 4)
+#pragma unroll
+          for (int box = 0; box < 4; ++box)
+            if (box < boxes)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + box * 8192 + r * 128), "r"(0) : "memory");
         fence_proxy_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&t->full[at]), 0));
@@ -360,8 +361,6 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
       const int f = c.f0 + int(rank) * 128 + quarter * 32 + 4 * (lane & 7);
       Bias4 bias{};
       if (kFinish && shape.splits == 1) bias = load_bias4(p.epi, p.m, f);
-      if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
-      tc_fence_after();
       const bool summed = c.step1 > c.step0;
       const uint32_t lanes = tmem + buf * 256 + (uint32_t(quarter * 32) << 16);
       const int chunks = (c.valid + 15) >> 4;
@@ -403,21 +402,69 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
         if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&t->acc_empty[buf]), 0));
         released = true;
       };
-      for (int k = first_chunk; k < chunks; k += 4) {
-        uint32_t va[16], vb[16];
-        const bool two = k + 2 < chunks;
-        Residual4<4> ra{}, rb{};
-        if (kFinish && shape.splits == 1) {
-          const int64_t row = c.out_row + k * 16 + (lane >> 3);
-          ra = load_residual4<4>(p.epi, p.m, row, 4, last, f, shape.vec);
-          if (two) rb = load_residual4<4>(p.epi, p.m, row + 32, 4, last, f, shape.vec);
+      if (!kFinish && shape.vec8 && summed) {
+        if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
+        tc_fence_after();
+        // 16-bit sums and nothing else: two chunks at a time, read as fragments of 8x8 matrices, rounded two output
+        // rows per instruction, transposed by stmatrix into 1 KiB each ([row][32 features], the 16-byte pieces of a
+        // row XOR-swizzled) and stored 8 features per thread
+        uint16_t* block = reinterpret_cast<uint16_t*>(turn);
+        const uint32_t st_addr = smem_u32(block) + uint32_t(lane & 7) * 64 + (uint32_t(lane >> 3) ^ ((lane >> 1) & 3u)) * 16;
+        const int f8 = c.f0 + int(rank) * 128 + quarter * 32 + (lane & 3) * 8;
+        for (int k = first_chunk; k < chunks; k += 4) {
+          uint32_t v[2][16];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (k + 2 * u < chunks) {
+              tmem_ld_frag16(lanes + (k + 2 * u) * 16, v[u]);
+              tmem_ld_frag16(lanes + (k + 2 * u) * 16 + (16u << 16), v[u] + 8);
+            }
+          tmem_ld_wait();
+          if (k + 4 >= chunks) release();
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t h[8];  // h[2m + t]: features 8m .., rows 8t .. of the chunk
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const int i = (m >> 1) * 8 + r * 4 + (m & 1) * 2;
+                h[2 * m + r] = pack_h16x2(__uint_as_float(v[u][i]), __uint_as_float(v[u][i + 1]), p.epi.fp16);
+              }
+            stmatrix_x4_trans(st_addr + u * 1024, h[0], h[2], h[4], h[6]);
+            stmatrix_x4_trans(st_addr + u * 1024 + 8 * 64, h[1], h[3], h[5], h[7]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int piece = lane + 32 * (i & 1);
+            const int row = (k + 2 * (i >> 1)) * 16 + (piece >> 2);
+            const uint4 q = *reinterpret_cast<const uint4*>(block + (i >> 1) * 512 + (piece >> 2) * 32 +
+                                                            ((piece & 3) ^ ((piece >> 3) & 3)) * 8);
+            if (row < c.valid && f8 < p.m)
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.epi.out) + (c.out_row + row) * p.m + f8) = q;
+          }
+          __syncwarp();
         }
-        tmem_ld16(lanes + k * 16, va);
-        if (two) tmem_ld16(lanes + (k + 2) * 16, vb);
-        tmem_ld_wait();
-        if (k + 4 >= chunks) release();
-        emit(k, va, ra);
-        if (two) emit(k + 2, vb, rb);
+      } else {
+        // a chunk's share of the residual is requested one chunk ahead
+        Residual4<4> res{};
+        const bool with_residual = kFinish && shape.splits == 1;
+        if (with_residual && first_chunk < chunks)
+          res = load_residual4<4>(p.epi, p.m, c.out_row + first_chunk * 16 + (lane >> 3), 4, last, f, shape.vec);
+        if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
+        tc_fence_after();
+        for (int k = first_chunk; k < chunks; k += 2) {
+          uint32_t v[16];
+          tmem_ld16(lanes + k * 16, v);
+          Residual4<4> next{};
+          if (with_residual && k + 2 < chunks)
+            next = load_residual4<4>(p.epi, p.m, c.out_row + (k + 2) * 16 + (lane >> 3), 4, last, f, shape.vec);
+          tmem_ld_wait();
+          if (k + 2 >= chunks) release();
+          emit(k, v, res);
+          res = next;
+        }
       }
       if (!released) release();
     }
@@ -525,6 +572,9 @@ int launch_product(ProductKind kind, const ProductArgs& args, void* workspace, i
   s.vec = args.m % 4 == 0 && aligned_to(e.out, e.out_fp32 ? 16 : 8) && (!e.slope || aligned_to(e.slope, 8)) &&
           (!e.residual || (aligned_to(e.residual, 8) && e.residual_pitch % 4 == 0));
 
+  const bool finish = e.bias || e.act || e.residual || e.slope;
+  s.vec8 = !finish && !e.out_fp32 && s.splits == 1 && args.m % 8 == 0 && aligned_to(e.out, 16);
+
   Maps maps;
   int rc;
   const int fp16 = e.fp16;
@@ -535,7 +585,6 @@ int launch_product(ProductKind kind, const ProductArgs& args, void* workspace, i
   for (int i = 0; i < kBoxes; ++i)
     if ((rc = make_map(&maps.b[i], args.b, weight ? args.n : args.k, args.rows, 1, args.b_pitch, 0, 16u << i, fp16))) return rc;
 
-  const bool finish = e.bias || e.act || e.residual || e.slope;
   const int variant = kind == kForward ? (finish ? 1 : 0) : kind == kInputGrad ? 2 : 3;
   const KernelFn kernel = kind == kForward     ? kernel_of<kForward>(finish)
                           : kind == kInputGrad ? kernel_of<kInputGrad>(false)
