@@ -515,13 +515,23 @@ _NORM_TYPES = {**_H16, torch.float32: PRECISION_FP32}
 def _h16(t: torch.Tensor, name: str) -> int:
     if not t.is_cuda:
         raise MB200Error(f"{name}: need a CUDA tensor, got one on {t.device}; there is no CPU path")
-    if t.dtype not in _H16:
+    precision = _H16.get(t.dtype)
+    if precision is None:
         raise MB200Error(f"{name}: need bf16 or fp16, got {t.dtype}")
-    return _H16[t.dtype]
+    return precision
+
+
+# A call through Python costs about as much as the smallest kernels take, so the common case (whole, contiguous tensors
+# on the current device) is told apart by a few attributes, and what is wrong is worked out only where something is.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = torch.cuda.current_device
 
 
 def _pitch(t: torch.Tensor, like: torch.Tensor, shape, name: str, dtypes=None) -> int:
     """Elements from row to row of a matrix whose columns lie side by side; refuses every other layout."""
+    if t.shape == shape and t.is_contiguous() and t.get_device() == like.get_device() and t.dtype in (dtypes or (like.dtype,)):
+        # the stride of a single row says nothing, and contiguous rows are as far apart as they are long
+        return shape[-1] if shape[-2] > 1 else (shape[-1] + 7) // 8 * 8
     dtypes = (like.dtype,) if dtypes is None else dtypes
     if t.dtype not in dtypes or t.device != like.device:
         raise MB200Error(f"{name}: need {' or '.join(map(str, dtypes))} on {like.device}, got {t.dtype} on {t.device}")
@@ -531,7 +541,7 @@ def _pitch(t: torch.Tensor, like: torch.Tensor, shape, name: str, dtypes=None) -
     if cols != 1 and t.stride(-1) != 1:
         raise MB200Error(f"{name}: the elements of a row must lie side by side, got strides {t.stride()}")
     if rows <= 1:
-        return (cols + 7) // 8 * 8  # the stride of a single row says nothing
+        return (cols + 7) // 8 * 8
     if t.stride(-2) < cols:
         raise MB200Error(f"{name}: rows overlap (strides {t.stride()})")
     return t.stride(-2)
@@ -540,15 +550,15 @@ def _pitch(t: torch.Tensor, like: torch.Tensor, shape, name: str, dtypes=None) -
 def _vector(t: Optional[torch.Tensor], like: torch.Tensor, n: int, name: str, dtypes) -> None:
     if t is None:
         return
-    if t.dtype not in dtypes or t.device != like.device or tuple(t.shape) != (n,) or not t.is_contiguous():
+    if t.dtype not in dtypes or t.get_device() != like.get_device() or t.shape != (n,) or not t.is_contiguous():
         raise MB200Error(f"{name}: need a contiguous vector of {n} elements of {' or '.join(map(str, dtypes))} on "
                          f"{like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _output(t: Optional[torch.Tensor], like: torch.Tensor, shape, dtype, name: str) -> torch.Tensor:
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    if t.dtype != dtype or t.device != like.device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        return like.new_empty(shape, dtype=dtype)
+    if t.dtype != dtype or t.get_device() != like.get_device() or t.shape != shape or not t.is_contiguous():
         raise MB200Error(f"{name}: need a contiguous tensor of {dtype} {tuple(shape)} on {like.device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     return t
@@ -557,25 +567,12 @@ def _output(t: Optional[torch.Tensor], like: torch.Tensor, shape, dtype, name: s
 def _scratch(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
     if nbytes < 0:
         raise MB200Error(load().mb200_last_error().decode())
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
-class _on_device:
-    """Makes a tensor's device the current one for a call."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, t: torch.Tensor) -> None:
-        self.index = t.device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _elsewhere(x: torch.Tensor) -> bool:
+    """Whether x lives on another GPU than the current one: the call is then made again with x's device current."""
+    return x.is_cuda and x.get_device() != _current_device()
 
 
 def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, out_dtype=None, want_slope: bool = False):
@@ -584,6 +581,9 @@ def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, o
     Rows may be further apart than they are long (a multiple of 8 elements); ``k`` is a multiple of 8, ``n`` is free.
     ``out`` may be the residual itself.  With ``want_slope`` also returns ``act'(x @ w.T + bias)`` in x's type, which
     ``linear_backward`` takes."""
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return linear(x, w, bias, activation, residual, out, out_dtype, want_slope)
     precision = _h16(x, "x")
     if x.dim() != 2 or w.dim() != 2:
         raise MB200Error(f"linear: need matrices, got x {tuple(x.shape)} and w {tuple(w.shape)}")
@@ -598,18 +598,15 @@ def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, o
     if out_dtype not in (x.dtype, torch.float32):
         raise MB200Error(f"linear: output of {out_dtype} for operands of {x.dtype}")
     y = _output(out, x, (rows, n), out_dtype, "out")
-    slope = torch.empty((rows, n), dtype=x.dtype, device=x.device) if want_slope else None
-    lib = load()
-    with _on_device(x):
-        ws = _scratch(lib.mb200_linear_workspace_bytes(rows, n, k, x.device.index), x)
-        _check(
-            lib.mb200_linear(
-                precision, _ptr(x), xp, rows, _ptr(w), wp, n, k, _ptr(bias), bias is not None and bias.dtype == torch.float32,
-                ACTIVATIONS[activation], _ptr(residual), rp, _ptr(y), out_dtype == torch.float32, _ptr(slope), _ptr(ws),
-                0 if ws is None else ws.numel(), x.device.index, _stream(x.device),
-            ),
-            "linear",
-        )
+    slope = x.new_empty((rows, n)) if want_slope else None
+    lib, dev = load(), x.get_device()
+    ws = _scratch(lib.mb200_linear_workspace_bytes(rows, n, k, dev), x)
+    rc = lib.mb200_linear(
+        precision, x.data_ptr(), xp, rows, w.data_ptr(), wp, n, k, _ptr(bias), bias is not None and bias.dtype == torch.float32,
+        ACTIVATIONS[activation], _ptr(residual), rp, y.data_ptr(), out_dtype == torch.float32, _ptr(slope), _ptr(ws),
+        0 if ws is None else ws.numel(), dev, _raw_stream(dev),
+    )
+    _check(rc, "linear")
     return (y, slope) if want_slope else y
 
 
@@ -624,6 +621,9 @@ def linear_backward(dy, x, w, slope=None, dw_dtype=None, want_dx: bool = True, w
     """Gradients ``(dx, dw, db)`` of ``linear`` (None where not wanted; the residual's gradient is ``dy``).  ``slope``: what
     ``linear(..., want_slope=True)`` returned, None for no activation.  ``dy`` may be fp32 for bf16 operands.  ``dy * slope``
     is rounded to x's type once, for the products; ``db`` is its fp32 sum before that; ``dw`` has w's type, or fp32."""
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return linear_backward(dy, x, w, slope, dw_dtype, want_dx, want_dw, want_db)
     precision = _h16(x, "x")
     if x.dim() != 2 or w.dim() != 2:
         raise MB200Error(f"linear_backward: need matrices, got x {tuple(x.shape)} and w {tuple(w.shape)}")
@@ -635,20 +635,16 @@ def linear_backward(dy, x, w, slope=None, dw_dtype=None, want_dx: bool = True, w
     if slope is not None:
         _output(slope, x, (rows, n), x.dtype, "slope")
     dw_dtype = _dw_type(w, dw_dtype)
-    dx = torch.empty((rows, k), dtype=x.dtype, device=x.device) if want_dx else None
-    dw = torch.empty((n, k), dtype=dw_dtype, device=x.device) if want_dw else None
-    db = torch.empty(n, dtype=torch.float32, device=x.device) if want_db else None
-    lib = load()
-    with _on_device(x):
-        ws = _scratch(lib.mb200_linear_backward_workspace_bytes(rows, n, k, x.device.index), x)
-        _check(
-            lib.mb200_linear_backward(
-                precision, _ptr(dy), dy.dtype == torch.float32, dp, _ptr(slope), _ptr(x), xp, rows, _ptr(w), wp, n, k,
-                _ptr(dx), _ptr(dw), dw_dtype == torch.float32, _ptr(db), _ptr(ws), 0 if ws is None else ws.numel(),
-                x.device.index, _stream(x.device),
-            ),
-            "linear_backward",
-        )
+    dx = x.new_empty((rows, k)) if want_dx else None
+    dw = w.new_empty((n, k), dtype=dw_dtype) if want_dw else None
+    db = x.new_empty(n, dtype=torch.float32) if want_db else None
+    lib, dev = load(), x.get_device()
+    ws = _scratch(lib.mb200_linear_backward_workspace_bytes(rows, n, k, dev), x)
+    rc = lib.mb200_linear_backward(
+        precision, dy.data_ptr(), dy.dtype == torch.float32, dp, _ptr(slope), x.data_ptr(), xp, rows, w.data_ptr(), wp, n, k,
+        _ptr(dx), _ptr(dw), dw_dtype == torch.float32, _ptr(db), _ptr(ws), 0 if ws is None else ws.numel(), dev, _raw_stream(dev),
+    )
+    _check(rc, "linear_backward")
     return dx, dw, db
 
 
@@ -669,41 +665,42 @@ def grouped_linear(x, w, offsets, out=None):
     """``x[r] @ w[e].T`` for the rows of segment e = ``offsets[e] .. offsets[e + 1] - 1``, of any length: x [rows, k] and
     w [experts, n, k] of bf16 or fp16, offsets [experts + 1] int32 on x's device (``align(..., pad_rows=1)`` returns them as
     ``mtile_prefix``).  Rows outside the segments are left as they are in ``out``, undefined in a tensor made here."""
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return grouped_linear(x, w, offsets, out)
     precision = _h16(x, "x")
     e, n, k, wp, ep = _expert_weight(w, x, offsets)
     rows = x.shape[0]
     xp = _pitch(x, x, (rows, k), "x")
     y = _output(out, x, (rows, n), x.dtype, "out")
-    with _on_device(x):
-        _check(
-            load().mb200_grouped_linear(precision, _ptr(x), xp, rows, _ptr(w), wp, ep, _ptr(offsets), e, n, k, _ptr(y),
-                                        x.device.index, _stream(x.device)),
-            "grouped_linear",
-        )
+    dev = x.get_device()
+    rc = load().mb200_grouped_linear(precision, x.data_ptr(), xp, rows, w.data_ptr(), wp, ep, offsets.data_ptr(), e, n, k,
+                                     y.data_ptr(), dev, _raw_stream(dev))
+    _check(rc, "grouped_linear")
     return y
 
 
 def grouped_linear_backward(dy, x, w, offsets, dw_dtype=None, dx_out=None, want_dx: bool = True, want_dw: bool = True):
     """Gradients ``(dx, dw)`` of ``grouped_linear`` (None where not wanted).  Rows outside the segments have no part in
     ``dw`` and are left as they are in ``dx_out``; an expert without rows gets a zero gradient.  ``dw`` has w's type, or fp32."""
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return grouped_linear_backward(dy, x, w, offsets, dw_dtype, dx_out, want_dx, want_dw)
     precision = _h16(x, "x")
     e, n, k, wp, ep = _expert_weight(w, x, offsets)
     rows = x.shape[0]
     xp, dp = _pitch(x, x, (rows, k), "x"), _pitch(dy, x, (rows, n), "dy")
     dw_dtype = _dw_type(w, dw_dtype)
     dx = _output(dx_out, x, (rows, k), x.dtype, "dx_out") if want_dx else None
-    dw = torch.empty((e, n, k), dtype=dw_dtype, device=x.device) if want_dw else None
-    lib = load()
-    with _on_device(x):
-        copied = dp % 8 or dy.data_ptr() % 16
-        ws = _scratch(lib.mb200_grouped_linear_backward_workspace_bytes(rows, n), x) if copied else None
-        _check(
-            lib.mb200_grouped_linear_backward(
-                precision, _ptr(dy), dp, _ptr(x), xp, rows, _ptr(w), wp, ep, _ptr(offsets), e, n, k, _ptr(dx), _ptr(dw),
-                dw_dtype == torch.float32, _ptr(ws), 0 if ws is None else ws.numel(), x.device.index, _stream(x.device),
-            ),
-            "grouped_linear_backward",
-        )
+    dw = w.new_empty((e, n, k), dtype=dw_dtype) if want_dw else None
+    lib, dev = load(), x.get_device()
+    copied = dp % 8 or dy.data_ptr() % 16
+    ws = _scratch(lib.mb200_grouped_linear_backward_workspace_bytes(rows, n), x) if copied else None
+    rc = lib.mb200_grouped_linear_backward(
+        precision, dy.data_ptr(), dp, x.data_ptr(), xp, rows, w.data_ptr(), wp, ep, offsets.data_ptr(), e, n, k, _ptr(dx), _ptr(dw),
+        dw_dtype == torch.float32, _ptr(ws), 0 if ws is None else ws.numel(), dev, _raw_stream(dev),
+    )
+    _check(rc, "grouped_linear_backward")
     return dx, dw
 
 
@@ -719,56 +716,57 @@ def linear_status(device=None, clear: bool = False) -> int:
 def _norm_operands(x, weight, bias, name: str):
     if not x.is_cuda:
         raise MB200Error(f"{name}: need CUDA tensors, got one on {x.device}; there is no CPU path")
-    if x.dtype not in _NORM_TYPES:
+    precision = _NORM_TYPES.get(x.dtype)
+    if precision is None:
         raise MB200Error(f"{name}: need bf16, fp16 or fp32, got {x.dtype}")
     if x.dim() != 2 or x.shape[1] == 0:
         raise MB200Error(f"{name}: need x [rows, hidden], got {tuple(x.shape)}")
-    h = x.shape[1]
-    types = {t.dtype for t in (weight, bias) if t is not None}
-    if len(types) > 1:
-        raise MB200Error(f"{name}: weight and bias of one type, got {sorted(map(str, types))}")
-    for t, what in ((weight, "weight"), (bias, "bias")):
-        _vector(t, x, h, what, (x.dtype, torch.float32))
-    return _NORM_TYPES[x.dtype], x.shape[0], h, types == {torch.float32}
+    rows, h = x.shape
+    _vector(weight, x, h, "weight", (x.dtype, torch.float32))
+    _vector(bias, x, h, "bias", (x.dtype, torch.float32))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise MB200Error(f"{name}: weight and bias of one type, got {weight.dtype} and {bias.dtype}")
+    params = weight if weight is not None else bias
+    return precision, rows, h, params is not None and params.dtype == torch.float32
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     """Layer norm of the rows of ``x [rows, hidden]`` (bf16, fp16 or fp32; rows may be any distance apart): returns
     ``(y, mean, rstd)``, the last two in fp32 for ``layer_norm_backward``.  weight and bias have x's type or fp32."""
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return layer_norm(x, weight, bias, eps, out)
     precision, rows, h, fp32 = _norm_operands(x, weight, bias, "layer_norm")
     xp = _pitch(x, x, (rows, h), "x")
     y = _output(out, x, (rows, h), x.dtype, "out")
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
-    with _on_device(x):
-        _check(
-            load().mb200_layer_norm(precision, _ptr(x), xp, rows, h, _ptr(weight), _ptr(bias), fp32, eps, _ptr(y), _ptr(mean),
-                                    _ptr(rstd), x.device.index, _stream(x.device)),
-            "layer_norm",
-        )
+    mean, rstd = x.new_empty((2, rows), dtype=torch.float32).unbind()
+    dev = x.get_device()
+    rc = load().mb200_layer_norm(precision, x.data_ptr(), xp, rows, h, _ptr(weight), _ptr(bias), fp32, eps, y.data_ptr(),
+                                 mean.data_ptr(), rstd.data_ptr(), dev, _raw_stream(dev))
+    _check(rc, "layer_norm")
     return y, mean, rstd
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
     """Gradients ``(dx, dweight, dbias)`` of ``layer_norm`` (None where not wanted); the last two are fp32 sums over the rows,
     in a fixed order."""
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return layer_norm_backward(dy, x, mean, rstd, weight, want_dx, want_dweight, want_dbias)
     precision, rows, h, fp32 = _norm_operands(x, weight, None, "layer_norm_backward")
     xp, dp = _pitch(x, x, (rows, h), "x"), _pitch(dy, x, (rows, h), "dy")
     for t, what in ((mean, "mean"), (rstd, "rstd")):
         _vector(t, x, rows, what, (torch.float32,))
-    dx = torch.empty((rows, h), dtype=x.dtype, device=x.device) if want_dx else None
-    dweight = torch.empty(h, dtype=torch.float32, device=x.device) if want_dweight else None
-    dbias = torch.empty(h, dtype=torch.float32, device=x.device) if want_dbias else None
-    lib = load()
-    with _on_device(x):
-        ws = None
-        if want_dweight or want_dbias:
-            ws = _scratch(lib.mb200_layer_norm_backward_workspace_bytes(rows, h, x.device.index), x)
-        _check(
-            lib.mb200_layer_norm_backward(
-                precision, _ptr(dy), dp, _ptr(x), xp, rows, h, _ptr(mean), _ptr(rstd), _ptr(weight), fp32, _ptr(dx),
-                _ptr(dweight), _ptr(dbias), _ptr(ws), 0 if ws is None else ws.numel(), x.device.index, _stream(x.device),
-            ),
-            "layer_norm_backward",
-        )
+    dx = x.new_empty((rows, h)) if want_dx else None
+    dweight = x.new_empty(h, dtype=torch.float32) if want_dweight else None
+    dbias = x.new_empty(h, dtype=torch.float32) if want_dbias else None
+    lib, dev = load(), x.get_device()
+    ws = None
+    if want_dweight or want_dbias:
+        ws = _scratch(lib.mb200_layer_norm_backward_workspace_bytes(rows, h, dev), x)
+    rc = lib.mb200_layer_norm_backward(
+        precision, dy.data_ptr(), dp, x.data_ptr(), xp, rows, h, mean.data_ptr(), rstd.data_ptr(), _ptr(weight), fp32, _ptr(dx),
+        _ptr(dweight), _ptr(dbias), _ptr(ws), 0 if ws is None else ws.numel(), dev, _raw_stream(dev),
+    )
+    _check(rc, "layer_norm_backward")
     return dx, dweight, dbias

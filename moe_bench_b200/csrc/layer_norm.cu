@@ -5,6 +5,8 @@
 //
 // Statistics, gradients of the parameters and everything in between are fp32; y and dx are rounded once.
 
+#include <algorithm>
+
 #include "../../include/moe_bench_b200.h"
 #include "layer.cuh"
 
@@ -19,6 +21,7 @@ struct NormArgs {
   int64_t rows, hidden;
   const void* weight;   // null: 1
   const void* bias;     // null: 0
+  int params_fp32;
   float eps;
   void* out;            // y or dx, dense; backward: null if not wanted
   float* mean;
@@ -56,10 +59,305 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
   return s;
 }
 
+// ---- rows that fit the registers of a block ---------------------------------------------------------
+// A row is kPer vectors of kVec elements in each of blockDim.x threads; blockDim.y rows per block (more than one only
+// where a row takes a single warp).  x (and dy) are read once, the next row's while this one is reduced; a thread has
+// the same columns of every row, so its parameters stay in registers.  HBM is the bound, but 16-bit rows come close to
+// the issue slots (two elements per 32-bit word to take apart and put together), so all arithmetic is on pairs of
+// fp32 (f32x2) and every element is taken apart once: 951 instructions per warp and row of 7168 became about 400.
+
+// kVec elements side by side, as one access (16 bytes) or one element
+template <typename T, int kVec>
+struct alignas(sizeof(T) * kVec) Vec {
+  T v[kVec];
+};
+template <typename T, int kVec>
+__device__ __forceinline__ Vec<T, kVec> load_once(const T* p) {
+  Vec<T, kVec> r;
+  if constexpr (sizeof(T) * kVec == 16) {
+    *reinterpret_cast<uint4*>(&r) = __ldcs(reinterpret_cast<const uint4*>(p));
+  } else if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint16_t*>(&r) = __ldcs(reinterpret_cast<const unsigned short*>(p));
+  } else {
+    *reinterpret_cast<float*>(&r) = __ldcs(reinterpret_cast<const float*>(p));
+  }
+  return r;
+}
+
+// Two fp32 values that an instruction works on together; each is rounded as it would be alone.
+using Pair = uint64_t;
+__device__ __forceinline__ Pair pair_of(float a, float b) { return pack_f32x2(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float sum_of(Pair p) {
+  float a, b;
+  unpack_f32x2(p, a, b);
+  return a + b;
+}
+
+// A thread's kPer vectors as pairs.
+template <typename T, int kVec, int kPer>
+__device__ __forceinline__ void take_apart(const Vec<T, kVec> (&v)[kPer], Pair (&out)[kVec * kPer / 2]) {
+  if constexpr (kVec == 1) {
+#pragma unroll
+    for (int k = 0; k < kPer; k += 2) out[k / 2] = pair_of(to_float(v[k].v[0]), to_float(v[k + 1].v[0]));
+  } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&v[k]);
+#pragma unroll
+      for (int i = 0; i < kVec / 2; ++i) {
+        if constexpr (sizeof(T) == 2 && __is_same(T, __half)) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(w + i));
+          out[k * kVec / 2 + i] = pair_of(f.x, f.y);
+        } else {
+          out[k * kVec / 2 + i] = pack_f32x2(w[i] << 16, w[i] & 0xffff0000u);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+#pragma unroll
+      for (int i = 0; i < kVec / 2; ++i) out[k * kVec / 2 + i] = pair_of(v[k].v[2 * i], v[k].v[2 * i + 1]);
+  }
+}
+
+template <typename T, int kVec, int kPer>
+__device__ __forceinline__ void store_row(T* row, int64_t hidden, const Pair (&p)[kVec * kPer / 2]) {
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int64_t at = int64_t(threadIdx.x + k * blockDim.x) * kVec;
+    if (at < hidden) {
+      Vec<T, kVec> o;
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const int e = k * kVec + i;
+        float f[2];
+        unpack_f32x2(p[e / 2], f[0], f[1]);
+        if constexpr (sizeof(T) == 2 && kVec > 1) {
+          if (i % 2 == 0) reinterpret_cast<uint32_t*>(&o)[i / 2] = pack_h16x2(f[0], f[1], __is_same(T, __half));
+        } else {
+          o.v[i] = from_float<T>(f[e & 1]);
+        }
+      }
+      *reinterpret_cast<Vec<T, kVec>*>(row + at) = o;
+    }
+  }
+}
+
+// Parameters of this thread's columns, of T or fp32; `other` where there are none and past the row's end.
+template <typename T, int kVec, int kPer>
+__device__ __forceinline__ void load_params(const void* p, int fp32, int64_t hidden, float other, Pair (&out)[kVec * kPer / 2]) {
+  float f[kVec * kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int64_t at = int64_t(threadIdx.x + k * blockDim.x) * kVec;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) f[k * kVec + i] = other;
+    if (p == nullptr || at >= hidden) continue;
+    if (fp32) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) f[k * kVec + i] = __ldg(reinterpret_cast<const float*>(p) + at + i);
+    } else {
+      const Vec<T, kVec> r = *reinterpret_cast<const Vec<T, kVec>*>(reinterpret_cast<const T*>(p) + at);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) f[k * kVec + i] = to_float(r.v[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kVec * kPer / 2; ++i) out[i] = pair_of(f[2 * i], f[2 * i + 1]);
+}
+
+// Sums of kCount values over a row's threads, the same in all of them.  The calls of a block take the two halves of
+// `part` in turn, so that one barrier is enough.
+template <int kCount>
+__device__ __forceinline__ void row_sums(float (&v)[kCount], float (*part)[32][2], int& turn) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int c = 0; c < kCount; ++c) v[c] += __shfl_xor_sync(0xffffffffu, v[c], o);
+  if (blockDim.x == 32) return;
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (lane == 0)
+#pragma unroll
+    for (int c = 0; c < kCount; ++c) part[turn][threadIdx.x >> 5][c] = v[c];
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < kCount; ++c) v[c] = lane < warps ? part[turn][lane][c] : 0.f;
+  turn ^= 1;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int c = 0; c < kCount; ++c) v[c] += __shfl_xor_sync(0xffffffffu, v[c], o);
+}
+
+// Columns past the row's end read as zero.
+template <typename T, int kVec, int kPer>
+__device__ __forceinline__ void load_row(const void* base, int64_t pitch, int64_t row, int64_t rows, int64_t hidden,
+                                         Vec<T, kVec> (&v)[kPer]) {
+  const T* p = reinterpret_cast<const T*>(base) + row * pitch;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int64_t at = int64_t(threadIdx.x + k * blockDim.x) * kVec;
+    v[k] = Vec<T, kVec>{};
+    if (row < rows && at < hidden) v[k] = load_once<T, kVec>(p + at);
+  }
+}
+
+template <typename T, int kVec, int kPer, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads) norm_kernel(const NormArgs p) {
+  constexpr int kPairs = kVec * kPer / 2;
+  __shared__ float part[2][32][2];
+  int turn = 0;
+  const int64_t step = int64_t(gridDim.x) * blockDim.y;
+  const float inv = 1.f / float(p.hidden);
+  int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+  Vec<T, kVec> x[kPer];
+  load_row<T, kVec, kPer>(p.x, p.x_pitch, r, p.rows, p.hidden, x);
+  Pair w[kPairs], b[kPairs];
+  load_params<T, kVec, kPer>(p.weight, p.params_fp32, p.hidden, 1.f, w);
+  load_params<T, kVec, kPer>(p.bias, p.params_fp32, p.hidden, 0.f, b);
+  // all rows of a block take the same number of turns: its threads meet at the barriers
+  for (int64_t first = int64_t(blockIdx.x) * blockDim.y; first < p.rows; first += step, r += step) {
+    Pair d[kPairs];
+    take_apart<T, kVec, kPer>(x, d);
+    load_row<T, kVec, kPer>(p.x, p.x_pitch, r + step, p.rows, p.hidden, x);
+    Pair s2 = 0;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) s2 = add2(s2, d[i]);
+    float s[1] = {sum_of(s2)};
+    row_sums(s, part, turn);
+    const float mean = s[0] * inv;
+    const Pair m2 = pair_of(-mean, -mean);
+    s2 = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const bool inside = int64_t(threadIdx.x + k * blockDim.x) * kVec < p.hidden;
+      if constexpr (kVec == 1) {
+        const bool second = int64_t(threadIdx.x + (k + 1) * blockDim.x) < p.hidden;
+        if (k % 2 == 0) {
+          float a, c;
+          unpack_f32x2(add2(d[k / 2], m2), a, c);
+          d[k / 2] = pair_of(inside ? a : 0.f, second ? c : 0.f);
+          s2 = fma2(d[k / 2], d[k / 2], s2);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVec / 2; ++i) {
+          Pair& e = d[k * kVec / 2 + i];
+          e = inside ? add2(e, m2) : 0;
+          s2 = fma2(e, e, s2);
+        }
+      }
+    }
+    s[0] = sum_of(s2);
+    row_sums(s, part, turn);
+    const float rstd = 1.f / sqrtf(s[0] * inv + p.eps);
+    if (r < p.rows) {
+      const Pair r2 = pair_of(rstd, rstd);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) d[i] = fma2(mul2(d[i], r2), w[i], b[i]);
+      store_row<T, kVec, kPer>(reinterpret_cast<T*>(p.out) + r * p.hidden, p.hidden, d);
+      if (threadIdx.x == 0) {
+        p.mean[r] = mean;
+        p.rstd[r] = rstd;
+      }
+    }
+  }
+}
+
+// Every thread keeps the sums of its columns over the rows it sees, and leaves them in `sums` at the end.  Columns past
+// the row's end have dy = 0, so they add nothing to any sum.
+template <typename T, int kVec, int kPer, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads) norm_grad_kernel(const NormArgs p) {
+  constexpr int kPairs = kVec * kPer / 2;
+  __shared__ float part[2][32][2];
+  int turn = 0;
+  const int64_t step = int64_t(gridDim.x) * blockDim.y;
+  const float inv = 1.f / float(p.hidden);
+  int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+  Vec<T, kVec> x[kPer], dy[kPer];
+  load_row<T, kVec, kPer>(p.x, p.x_pitch, r, p.rows, p.hidden, x);
+  load_row<T, kVec, kPer>(p.dy, p.dy_pitch, r, p.rows, p.hidden, dy);
+  float mean = r < p.rows ? __ldg(p.mean + r) : 0.f, rstd = r < p.rows ? __ldg(p.rstd + r) : 0.f;
+  Pair w[kPairs], dw[kPairs] = {}, db[kPairs] = {};
+  load_params<T, kVec, kPer>(p.weight, p.params_fp32, p.hidden, 1.f, w);
+  for (int64_t first = int64_t(blockIdx.x) * blockDim.y; first < p.rows; first += step, r += step) {
+    Pair h[kPairs], g[kPairs];
+    take_apart<T, kVec, kPer>(x, h);
+    take_apart<T, kVec, kPer>(dy, g);
+    const Pair m2 = pair_of(-mean, -mean), r2 = pair_of(rstd, rstd);
+    const bool here = r < p.rows;
+    const bool more = r + step < p.rows;
+    load_row<T, kVec, kPer>(p.x, p.x_pitch, r + step, p.rows, p.hidden, x);
+    load_row<T, kVec, kPer>(p.dy, p.dy_pitch, r + step, p.rows, p.hidden, dy);
+    mean = more ? __ldg(p.mean + r + step) : 0.f;
+    rstd = more ? __ldg(p.rstd + r + step) : 0.f;
+    Pair sg = 0, sgh = 0;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      h[i] = mul2(add2(h[i], m2), r2);
+      dw[i] = fma2(g[i], h[i], dw[i]);
+      db[i] = add2(db[i], g[i]);
+      g[i] = mul2(g[i], w[i]);
+      sg = add2(sg, g[i]);
+      sgh = fma2(g[i], h[i], sgh);
+    }
+    if (p.out) {
+      float s[2] = {sum_of(sg), sum_of(sgh)};
+      row_sums(s, part, turn);
+      if (here) {
+        const Pair a2 = pair_of(-s[0] * inv, -s[0] * inv), b2 = pair_of(-s[1] * inv, -s[1] * inv);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) g[i] = mul2(r2, fma2(h[i], b2, add2(g[i], a2)));
+        store_row<T, kVec, kPer>(reinterpret_cast<T*>(p.out) + r * p.hidden, p.hidden, g);
+      }
+    }
+  }
+  if (p.sums == nullptr) return;
+  float* sums = p.sums + (int64_t(blockIdx.x) * blockDim.y + threadIdx.y) * 2 * p.hidden;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int64_t at = int64_t(threadIdx.x + k * blockDim.x) * kVec;
+    if (at < p.hidden) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const int e = k * kVec + i;
+        float f[2];
+        unpack_f32x2(dw[e / 2], f[0], f[1]);
+        sums[at + i] = f[e & 1];
+        unpack_f32x2(db[e / 2], f[0], f[1]);
+        sums[p.hidden + at + i] = f[e & 1];
+      }
+    }
+  }
+}
+
+// ---- rows of any length ------------------------------------------------------------------------------
 constexpr int kLongThreads = 512;
 
-// Rows of any length: a block per row, the row read once per pass.
-template <typename T, typename P>
+template <typename T>
+__device__ __forceinline__ float param(const void* p, int fp32, int64_t i, float other) {
+  if (p == nullptr) return other;
+  return fp32 ? __ldg(reinterpret_cast<const float*>(p) + i) : to_float(reinterpret_cast<const T*>(p)[i]);
+}
+
+// A block per row, the row read once per pass.
+template <typename T>
 __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const NormArgs p) {
   __shared__ float part[kLongThreads / 32];
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
@@ -75,10 +373,8 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const NormArgs 
     const float rstd = 1.f / sqrtf(block_sum(s, part) / float(p.hidden) + p.eps);
     T* y = reinterpret_cast<T*>(p.out) + r * p.hidden;
     for (int64_t i = threadIdx.x; i < p.hidden; i += kLongThreads) {
-      float v = (to_float(x[i]) - mean) * rstd;
-      if (p.weight) v *= to_float(reinterpret_cast<const P*>(p.weight)[i]);
-      if (p.bias) v += to_float(reinterpret_cast<const P*>(p.bias)[i]);
-      y[i] = from_float<T>(v);
+      y[i] = from_float<T>(fmaf((to_float(x[i]) - mean) * rstd, param<T>(p.weight, p.params_fp32, i, 1.f),
+                                param<T>(p.bias, p.params_fp32, i, 0.f)));
     }
     if (threadIdx.x == 0) {
       p.mean[r] = mean;
@@ -87,7 +383,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const NormArgs 
   }
 }
 
-template <typename T, typename P>
+template <typename T>
 __global__ void __launch_bounds__(kLongThreads) norm_grad_long_kernel(const NormArgs p) {
   __shared__ float part[kLongThreads / 32];
   float* sums = p.sums ? p.sums + int64_t(blockIdx.x) * 2 * p.hidden : nullptr;
@@ -98,7 +394,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_grad_long_kernel(const Norm
     float sg = 0.f, sgh = 0.f;
     for (int64_t i = threadIdx.x; i < p.hidden; i += kLongThreads) {
       const float d = to_float(dy[i]);
-      const float g = p.weight ? d * to_float(reinterpret_cast<const P*>(p.weight)[i]) : d;
+      const float g = d * param<T>(p.weight, p.params_fp32, i, 1.f);
       sg += g;
       sgh = fmaf(g, (to_float(x[i]) - mean) * rstd, sgh);
     }
@@ -110,7 +406,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_grad_long_kernel(const Norm
     for (int64_t i = threadIdx.x; i < p.hidden; i += kLongThreads) {
       const float d = to_float(dy[i]);
       const float h = (to_float(x[i]) - mean) * rstd;
-      const float g = p.weight ? d * to_float(reinterpret_cast<const P*>(p.weight)[i]) : d;
+      const float g = d * param<T>(p.weight, p.params_fp32, i, 1.f);
       if (dx) dx[i] = from_float<T>(rstd * (g - sg - h * sgh));
       if (sums) {  // this thread's own column of this block's own sums
         const bool first = r == blockIdx.x;
@@ -121,13 +417,20 @@ __global__ void __launch_bounds__(kLongThreads) norm_grad_long_kernel(const Norm
   }
 }
 
-// dweight and dbias: the blocks' sums added in block order.
-__global__ void __launch_bounds__(256) norm_param_grad_kernel(const float* sums, int blocks, int64_t hidden, float* dweight,
+// dweight and dbias: the parts added in a fixed order, 32 columns x 8 lanes per block.
+__global__ void __launch_bounds__(256) norm_param_grad_kernel(const float* sums, int parts, int64_t hidden, float* dweight,
                                                               float* dbias) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= 2 * hidden) return;
+  __shared__ float lanes[8][32];
+  const int c = threadIdx.x & 31, lane = threadIdx.x >> 5;
+  const int64_t i = int64_t(blockIdx.x) * 32 + c;
   float s = 0.f;
-  for (int b = 0; b < blocks; ++b) s += sums[int64_t(b) * 2 * hidden + i];
+  if (i < 2 * hidden)
+#pragma unroll 8
+    for (int b = lane; b < parts; b += 8) s += sums[int64_t(b) * 2 * hidden + i];
+  lanes[lane][c] = s;
+  __syncthreads();
+  if (lane != 0 || i >= 2 * hidden) return;
+  for (int k = 1; k < 8; ++k) s += lanes[k][c];
   if (i < hidden) {
     if (dweight) dweight[i] = s;
   } else if (dbias) {
@@ -135,10 +438,105 @@ __global__ void __launch_bounds__(256) norm_param_grad_kernel(const float* sums,
   }
 }
 
-int grid_blocks(int64_t rows, int device) {
-  const int sms = device_sm_count(device);
-  const int64_t most = int64_t(sms > 0 ? sms : 1) * 4;
-  return int(rows < most ? rows : most);
+// How a call runs: which kernel, its block and its grid.
+struct Plan {
+  int vec;      // elements per access, 0: the kernel for rows of any length
+  int per;      // vectors per thread
+  int most;     // threads the kernel is built for
+  dim3 block;
+  int blocks;
+  int parts;    // sums per column that the blocks of the backward kernel leave
+};
+
+// The register kernels: vectors (or single elements) per thread, threads at most, blocks that an SM's registers hold
+// for each thread of a block (65536 / registers).
+struct Shape {
+  int per, most, threads_per_sm;
+};
+constexpr Shape kForwardVec[] = {{1, 512, 1024}, {2, 512, 1024}, {4, 512, 512}};
+constexpr Shape kForwardVecFew[] = {{1, 1024, 1024}, {2, 1024, 1024}, {4, 512, 512}};
+constexpr Shape kForwardOne[] = {{4, 256, 1024}, {16, 1024, 1024}};
+constexpr Shape kForwardOneFew[] = {{4, 1024, 1024}, {16, 1024, 1024}};
+constexpr Shape kBackwardVec[] = {{1, 512, 1024}, {2, 512, 512}};
+constexpr Shape kBackwardVecFew[] = {{1, 1024, 1024}, {2, 512, 512}};
+constexpr Shape kBackwardOne[] = {{4, 512, 1024}, {16, 512, 512}};
+constexpr Shape kBackwardOneFew[] = {{4, 1024, 1024}, {16, 512, 512}};
+constexpr Shape kBackwardVec32 = {4, 512, 512};  // fp32 only: 16-bit rows of that length spill their sums
+
+template <size_t kCount>
+bool pick(const Shape (&shapes)[kCount], int64_t vecs, Shape& out) {
+  for (const Shape& s : shapes)
+    if (vecs <= int64_t(s.per) * s.most) {
+      out = s;
+      return true;
+    }
+  return false;
+}
+
+// Few rows (each SM gets one at most): as many threads as there are, for latency; many: few threads that keep
+// several loads each in flight.
+Plan make_plan(bool backward, int elem_bytes, bool aligned, int64_t rows, int64_t hidden, int device) {
+  const int sms = device_sm_count(device) > 0 ? device_sm_count(device) : 1;
+  Plan l{};
+  l.vec = aligned ? 16 / elem_bytes : 1;
+  const int64_t vecs = (hidden + l.vec - 1) / l.vec;
+  Shape s;
+  const bool few = rows <= sms;
+  bool found = backward ? (aligned ? (few ? pick(kBackwardVecFew, vecs, s) : pick(kBackwardVec, vecs, s))
+                                         : (few ? pick(kBackwardOneFew, vecs, s) : pick(kBackwardOne, vecs, s)))
+                              : (aligned ? (few ? pick(kForwardVecFew, vecs, s) : pick(kForwardVec, vecs, s))
+                                         : (few ? pick(kForwardOneFew, vecs, s) : pick(kForwardOne, vecs, s)));
+  if (!found && backward && aligned && elem_bytes == 4 && vecs <= kBackwardVec32.per * kBackwardVec32.most) {
+    s = kBackwardVec32;
+    found = true;
+  }
+  if (!found) {
+    l.vec = 0;
+    l.block = dim3(kLongThreads);
+    l.blocks = int(rows < 2 * sms ? rows : 2 * sms);
+    l.parts = l.blocks;
+    return l;
+  }
+  l.per = s.per;
+  l.most = s.most;
+  const int tpr = int((vecs + l.per - 1) / l.per + 31) / 32 * 32;
+  l.block = dim3(tpr, tpr == 32 ? 8 : 1);
+  const int threads = tpr * int(l.block.y);
+  int resident = s.threads_per_sm / threads;
+  resident = resident < 1 ? 1 : resident;
+  const int64_t wanted = (rows + l.block.y - 1) / l.block.y;
+  l.blocks = int(wanted < int64_t(sms) * resident ? wanted : int64_t(sms) * resident);
+  l.parts = l.blocks * int(l.block.y);
+  return l;
+}
+
+template <typename T>
+void launch_forward(const NormArgs& a, const Plan& l, cudaStream_t s) {
+  constexpr int kV = 16 / sizeof(T);
+  if (l.vec == 0) norm_long_kernel<T><<<l.blocks, l.block, 0, s>>>(a);
+  else if (l.vec == 1 && l.per == 4) norm_kernel<T, 1, 4, 1024><<<l.blocks, l.block, 0, s>>>(a);
+  else if (l.vec == 1) norm_kernel<T, 1, 16, 1024><<<l.blocks, l.block, 0, s>>>(a);
+  else if (l.per == 1) norm_kernel<T, kV, 1, 1024><<<l.blocks, l.block, 0, s>>>(a);
+  else if (l.per == 2) norm_kernel<T, kV, 2, 1024><<<l.blocks, l.block, 0, s>>>(a);
+  else norm_kernel<T, kV, 4, 512><<<l.blocks, l.block, 0, s>>>(a);
+}
+template <typename T>
+void launch_backward(const NormArgs& a, const Plan& l, cudaStream_t s) {
+  constexpr int kV = 16 / sizeof(T);
+  if (l.vec == 0) norm_grad_long_kernel<T><<<l.blocks, l.block, 0, s>>>(a);
+  else if (l.vec == 1 && l.per == 4) norm_grad_kernel<T, 1, 4, 1024><<<l.blocks, l.block, 0, s>>>(a);
+  else if (l.vec == 1) norm_grad_kernel<T, 1, 16, 512><<<l.blocks, l.block, 0, s>>>(a);
+  else if (l.per == 1) norm_grad_kernel<T, kV, 1, 1024><<<l.blocks, l.block, 0, s>>>(a);
+  else if (l.per == 2) norm_grad_kernel<T, kV, 2, 512><<<l.blocks, l.block, 0, s>>>(a);
+  else if constexpr (sizeof(T) == 4) norm_grad_kernel<T, kV, 4, 512><<<l.blocks, l.block, 0, s>>>(a);
+}
+
+// Whether every row of every tensor starts on a 16-byte boundary.
+bool rows_aligned(const NormArgs& a, int elem_bytes) {
+  auto at = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  const int64_t v = 16 / elem_bytes;
+  return a.hidden % v == 0 && a.x_pitch % v == 0 && (!a.dy || a.dy_pitch % v == 0) && at(a.x) && at(a.dy) && at(a.weight) &&
+         at(a.bias) && at(a.out);
 }
 
 int check_norm(int precision, int64_t rows, int64_t hidden, const char* what) {
@@ -148,15 +546,6 @@ int check_norm(int precision, int64_t rows, int64_t hidden, const char* what) {
                 (long long)hidden);
   MB200_REQUIRE(hidden <= (int64_t(1) << 30), kUnsupportedShape, "%s: hidden=%lld", what, (long long)hidden);
   return kOk;
-}
-
-template <typename T, typename P>
-void launch_forward(const NormArgs& a, int blocks, cudaStream_t s) {
-  norm_long_kernel<T, P><<<blocks, kLongThreads, 0, s>>>(a);
-}
-template <typename T, typename P>
-void launch_backward(const NormArgs& a, int blocks, cudaStream_t s) {
-  norm_grad_long_kernel<T, P><<<blocks, kLongThreads, 0, s>>>(a);
 }
 
 }  // namespace
@@ -183,24 +572,28 @@ int mb200_layer_norm(int precision, const void* x, int64_t x_pitch, int64_t rows
   a.hidden = hidden;
   a.weight = weight;
   a.bias = bias;
+  a.params_fp32 = params_fp32 != 0;
   a.eps = eps;
   a.out = y;
   a.mean = mean;
   a.rstd = rstd;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int blocks = grid_blocks(rows, device);
-  if (precision == MB200_PRECISION_FP32) launch_forward<float, float>(a, blocks, s);
-  else if (precision == MB200_PRECISION_FP16 && params_fp32) launch_forward<__half, float>(a, blocks, s);
-  else if (precision == MB200_PRECISION_FP16) launch_forward<__half, __half>(a, blocks, s);
-  else if (params_fp32) launch_forward<__nv_bfloat16, float>(a, blocks, s);
-  else launch_forward<__nv_bfloat16, __nv_bfloat16>(a, blocks, s);
+  const int size = precision == MB200_PRECISION_FP32 ? 4 : 2;
+  const Plan l = make_plan(false, size, rows_aligned(a, size), rows, hidden, device);
+  if (precision == MB200_PRECISION_FP32) launch_forward<float>(a, l, s);
+  else if (precision == MB200_PRECISION_FP16) launch_forward<__half>(a, l, s);
+  else launch_forward<__nv_bfloat16>(a, l, s);
   MB200_CHECK_CUDA(cudaGetLastError());
   return kOk;
 }
 
 int64_t mb200_layer_norm_backward_workspace_bytes(int64_t rows, int64_t hidden, int device) {
   if (check_norm(MB200_PRECISION_FP32, rows, hidden, "layer_norm_backward_workspace_bytes")) return -1;
-  return int64_t(grid_blocks(rows, device)) * 2 * hidden * 4;
+  // the most that any type and alignment needs
+  int parts = 0;
+  for (const int size : {2, 4})
+    for (const bool aligned : {false, true}) parts = std::max(parts, make_plan(true, size, aligned, rows, hidden, device).parts);
+  return int64_t(parts) * 2 * hidden * 4;
 }
 
 int mb200_layer_norm_backward(int precision, const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch,
@@ -220,7 +613,6 @@ int mb200_layer_norm_backward(int precision, const void* dy, int64_t dy_pitch, c
   }
   MB200_REQUIRE(dy && x && mean && rstd, kInvalidArgument, "layer_norm_backward: null pointer");
   if (!dx && !dweight && !dbias) return kOk;
-  const int blocks = grid_blocks(rows, device);
   NormArgs a{};
   a.x = x;
   a.dy = dy;
@@ -229,25 +621,26 @@ int mb200_layer_norm_backward(int precision, const void* dy, int64_t dy_pitch, c
   a.rows = rows;
   a.hidden = hidden;
   a.weight = weight;
+  a.params_fp32 = params_fp32 != 0;
   a.out = dx;
   a.mean = const_cast<float*>(mean);
   a.rstd = const_cast<float*>(rstd);
+  const int size = precision == MB200_PRECISION_FP32 ? 4 : 2;
+  const Plan l = make_plan(true, size, rows_aligned(a, size), rows, hidden, device);
   if (dweight || dbias) {
-    const int64_t need = int64_t(blocks) * 2 * hidden * 4;
+    const int64_t need = int64_t(l.parts) * 2 * hidden * 4;
     MB200_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, kInvalidArgument,
                   "layer_norm_backward: needs a 16-byte aligned workspace");
     MB200_REQUIRE(workspace_bytes >= need, kWorkspaceTooSmall, "layer_norm_backward: workspace %lld < %lld bytes",
                   (long long)workspace_bytes, (long long)need);
     a.sums = reinterpret_cast<float*>(workspace);
   }
-  if (precision == MB200_PRECISION_FP32) launch_backward<float, float>(a, blocks, s);
-  else if (precision == MB200_PRECISION_FP16 && params_fp32) launch_backward<__half, float>(a, blocks, s);
-  else if (precision == MB200_PRECISION_FP16) launch_backward<__half, __half>(a, blocks, s);
-  else if (params_fp32) launch_backward<__nv_bfloat16, float>(a, blocks, s);
-  else launch_backward<__nv_bfloat16, __nv_bfloat16>(a, blocks, s);
+  if (precision == MB200_PRECISION_FP32) launch_backward<float>(a, l, s);
+  else if (precision == MB200_PRECISION_FP16) launch_backward<__half>(a, l, s);
+  else launch_backward<__nv_bfloat16>(a, l, s);
   MB200_CHECK_CUDA(cudaGetLastError());
   if (a.sums) {
-    norm_param_grad_kernel<<<unsigned((2 * hidden + 255) / 256), 256, 0, s>>>(a.sums, blocks, hidden, dweight, dbias);
+    norm_param_grad_kernel<<<unsigned((2 * hidden + 31) / 32), 256, 0, s>>>(a.sums, l.parts, hidden, dweight, dbias);
     MB200_CHECK_CUDA(cudaGetLastError());
   }
   return kOk;
