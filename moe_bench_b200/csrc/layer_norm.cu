@@ -6,6 +6,7 @@
 // Statistics, gradients of the parameters and everything in between are fp32; y and dx are rounded once.
 
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/moe_bench_b200.h"
 #include "layer.cuh"
@@ -205,73 +206,179 @@ __device__ __forceinline__ void row_sums(float (&v)[kCount], float (*part)[32][2
     for (int c = 0; c < kCount; ++c) v[c] += __shfl_xor_sync(0xffffffffu, v[c], o);
 }
 
-// Columns past the row's end read as zero.
+// The rows of a thread on their way: kStages rows ahead in shared memory by cp.async, every thread its own vectors (so
+// that nothing but its own wait stands between copy and use), or where single elements are copied the next row in registers.
+// Columns past the row's end and rows past the last read as zero.
+constexpr int kStages = 3;
 template <typename T, int kVec, int kPer>
-__device__ __forceinline__ void load_row(const void* base, int64_t pitch, int64_t row, int64_t rows, int64_t hidden,
-                                         Vec<T, kVec> (&v)[kPer]) {
-  const T* p = reinterpret_cast<const T*>(base) + row * pitch;
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int64_t at = int64_t(threadIdx.x + k * blockDim.x) * kVec;
-    v[k] = Vec<T, kVec>{};
-    if (row < rows && at < hidden) v[k] = load_once<T, kVec>(p + at);
+struct RowStream {
+  static constexpr bool kShared = kVec > 1;
+  const T* base;
+  int64_t pitch, rows, hidden;
+  uint32_t slot;           // this thread's first vector of stage 0
+  uint32_t stage_bytes;
+  Vec<T, kVec> ahead[kShared ? 1 : kPer];
+
+  __device__ __forceinline__ RowStream(const void* p, int64_t pitch_, int64_t rows_, int64_t hidden_, uint32_t smem, int which, int streams)
+      : base(reinterpret_cast<const T*>(p)), pitch(pitch_), rows(rows_), hidden(hidden_) {
+    const uint32_t threads = blockDim.x * blockDim.y, thread = threadIdx.y * blockDim.x + threadIdx.x;
+    stage_bytes = threads * kPer * 16 * streams;
+    slot = smem + which * threads * kPer * 16 + thread * 16;
   }
+  __device__ __forceinline__ void request(int64_t row, int stage) {
+    const T* p = base + row * pitch;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int64_t at = int64_t(threadIdx.x + k * blockDim.x) * kVec;
+      const bool inside = row < rows && at < hidden;
+      if constexpr (kShared) {
+        const uint32_t to = slot + stage * stage_bytes + k * blockDim.x * blockDim.y * 16;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(inside ? p + at : base), "r"(inside ? 16 : 0)
+                     : "memory");
+      } else {
+        ahead[k] = Vec<T, kVec>{};
+        if (inside) ahead[k] = load_once<T, kVec>(p + at);
+      }
+    }
+  }
+  __device__ __forceinline__ void take(int stage, Pair (&out)[kVec * kPer / 2]) {
+    if constexpr (kShared) {
+      Vec<T, kVec> v[kPer];
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v[k]);
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(slot + stage * stage_bytes + k * blockDim.x * blockDim.y * 16)
+                     : "memory");
+      }
+      take_apart<T, kVec, kPer>(v, out);
+    } else {
+      take_apart<T, kVec, kPer>(ahead, out);
+    }
+  }
+};
+__device__ __forceinline__ void stream_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void stream_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
+
+// Which of a thread's vectors lie inside the row, and how many elements its warp and the warp with the number of its lane
+// have; the same for every row.
+template <int kVec, int kPer>
+struct RowShare {
+  uint32_t mask = 0;
+  float own_inv, there, there_inv;
+  static __device__ __forceinline__ float count(int warp, int64_t hidden) {
+    int64_t n = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int64_t left = hidden - int64_t(warp * 32 + k * blockDim.x) * kVec;
+      n += left <= 0 ? 0 : left < 32 * kVec ? left : 32 * kVec;
+    }
+    return float(n);
+  }
+  __device__ __forceinline__ explicit RowShare(int64_t hidden) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (int64_t(threadIdx.x + k * blockDim.x) * kVec < hidden) mask |= 1u << k;
+    const float own = count(threadIdx.x >> 5, hidden);
+    own_inv = own > 0.f ? 1.f / own : 0.f;
+    there = int(threadIdx.x & 31) < int(blockDim.x >> 5) ? count(threadIdx.x & 31, hidden) : 0.f;
+    there_inv = there > 0.f ? 1.f / there : 0.f;
+  }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
-template <typename T, int kVec, int kPer, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads) norm_kernel(const NormArgs p) {
+// Mean of a row and sum of the squares about it, with one exchange between its warps: each warp takes the squares about
+// its own mean, which are then moved to the common one, sum (x - m)^2 = sum over the warps of sum (x - m_w)^2 +
+// n_w (m_w - m)^2: terms that do not cancel, however far the row is from 0.
+template <int kVec, int kPer>
+__device__ __forceinline__ void row_moments(const Pair (&x)[kVec * kPer / 2], const RowShare<kVec, kPer>& share, float inv,
+                                            float (*part)[32][2], int& turn, float& mean, float& squares) {
   constexpr int kPairs = kVec * kPer / 2;
+  Pair s2 = 0;
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) s2 = add2(s2, x[i]);
+  const float s = warp_sum(sum_of(s2));
+  const float m = s * share.own_inv;
+  const Pair m2 = pair_of(-m, -m);
+  s2 = 0;
+  if constexpr (kVec == 1) {
+#pragma unroll
+    for (int k = 0; k < kPer; k += 2) {
+      float a, b;
+      unpack_f32x2(add2(x[k / 2], m2), a, b);
+      const Pair d = pair_of(share.mask >> k & 1 ? a : 0.f, share.mask >> (k + 1) & 1 ? b : 0.f);
+      s2 = fma2(d, d, s2);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (share.mask >> k & 1)
+#pragma unroll
+        for (int i = 0; i < kVec / 2; ++i) {
+          const Pair d = add2(x[k * kVec / 2 + i], m2);
+          s2 = fma2(d, d, s2);
+        }
+  }
+  const float q = warp_sum(sum_of(s2));
+  mean = m;
+  squares = q;
+  if (blockDim.x == 32) return;
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (lane == 0) {
+    part[turn][threadIdx.x >> 5][0] = s;
+    part[turn][threadIdx.x >> 5][1] = q;
+  }
+  __syncthreads();
+  const float ws = lane < warps ? part[turn][lane][0] : 0.f;
+  const float wq = lane < warps ? part[turn][lane][1] : 0.f;
+  turn ^= 1;
+  mean = warp_sum(ws) * inv;
+  const float off = ws * share.there_inv - mean;
+  squares = warp_sum(fmaf(share.there * off, off, wq));
+}
+
+template <typename T, int kVec, int kPer, int kMaxThreads, int kBlocks>
+__global__ void __launch_bounds__(kMaxThreads, kBlocks) norm_kernel(const NormArgs p) {
+  constexpr int kPairs = kVec * kPer / 2;
+  extern __shared__ __align__(16) uint8_t rows_smem[];
   __shared__ float part[2][32][2];
-  int turn = 0;
+  int turn = 0, stage = 0;
   const int64_t step = int64_t(gridDim.x) * blockDim.y;
   const float inv = 1.f / float(p.hidden);
   int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  Vec<T, kVec> x[kPer];
-  load_row<T, kVec, kPer>(p.x, p.x_pitch, r, p.rows, p.hidden, x);
+  using Stream = RowStream<T, kVec, kPer>;
+  constexpr int kAhead = Stream::kShared ? kStages : 1;
+  Stream x(p.x, p.x_pitch, p.rows, p.hidden, smem_u32(rows_smem), 0, 1);
+  for (int i = 0; i < kAhead; ++i) {
+    x.request(r + i * step, i);
+    stream_commit();
+  }
+  const RowShare<kVec, kPer> share(p.hidden);
   Pair w[kPairs], b[kPairs];
   load_params<T, kVec, kPer>(p.weight, p.params_fp32, p.hidden, 1.f, w);
   load_params<T, kVec, kPer>(p.bias, p.params_fp32, p.hidden, 0.f, b);
   // all rows of a block take the same number of turns: its threads meet at the barriers
   for (int64_t first = int64_t(blockIdx.x) * blockDim.y; first < p.rows; first += step, r += step) {
-    Pair d[kPairs];
-    take_apart<T, kVec, kPer>(x, d);
-    load_row<T, kVec, kPer>(p.x, p.x_pitch, r + step, p.rows, p.hidden, x);
-    Pair s2 = 0;
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) s2 = add2(s2, d[i]);
-    float s[1] = {sum_of(s2)};
-    row_sums(s, part, turn);
-    const float mean = s[0] * inv;
-    const Pair m2 = pair_of(-mean, -mean);
-    s2 = 0;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const bool inside = int64_t(threadIdx.x + k * blockDim.x) * kVec < p.hidden;
-      if constexpr (kVec == 1) {
-        const bool second = int64_t(threadIdx.x + (k + 1) * blockDim.x) < p.hidden;
-        if (k % 2 == 0) {
-          float a, c;
-          unpack_f32x2(add2(d[k / 2], m2), a, c);
-          d[k / 2] = pair_of(inside ? a : 0.f, second ? c : 0.f);
-          s2 = fma2(d[k / 2], d[k / 2], s2);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kVec / 2; ++i) {
-          Pair& e = d[k * kVec / 2 + i];
-          e = inside ? add2(e, m2) : 0;
-          s2 = fma2(e, e, s2);
-        }
-      }
-    }
-    s[0] = sum_of(s2);
-    row_sums(s, part, turn);
-    const float rstd = 1.f / sqrtf(s[0] * inv + p.eps);
+    Pair v[kPairs];
+    if (Stream::kShared) stream_wait();
+    x.take(stage, v);
+    x.request(r + kAhead * step, stage);
+    stream_commit();
+    stage = stage + 1 == kAhead ? 0 : stage + 1;
+    float mean, squares;
+    row_moments<kVec, kPer>(v, share, inv, part, turn, mean, squares);
+    const float rstd = 1.f / sqrtf(squares * inv + p.eps);
     if (r < p.rows) {
-      const Pair r2 = pair_of(rstd, rstd);
+      const Pair m2 = pair_of(-mean, -mean), r2 = pair_of(rstd, rstd);
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) d[i] = fma2(mul2(d[i], r2), w[i], b[i]);
-      store_row<T, kVec, kPer>(reinterpret_cast<T*>(p.out) + r * p.hidden, p.hidden, d);
+      for (int i = 0; i < kPairs; ++i) v[i] = fma2(mul2(add2(v[i], m2), r2), w[i], b[i]);
+      store_row<T, kVec, kPer>(reinterpret_cast<T*>(p.out) + r * p.hidden, p.hidden, v);
       if (threadIdx.x == 0) {
         p.mean[r] = mean;
         p.rstd[r] = rstd;
@@ -285,26 +392,36 @@ __global__ void __launch_bounds__(kMaxThreads) norm_kernel(const NormArgs p) {
 template <typename T, int kVec, int kPer, int kMaxThreads>
 __global__ void __launch_bounds__(kMaxThreads) norm_grad_kernel(const NormArgs p) {
   constexpr int kPairs = kVec * kPer / 2;
+  extern __shared__ __align__(16) uint8_t rows_smem[];
   __shared__ float part[2][32][2];
-  int turn = 0;
+  int turn = 0, stage = 0;
   const int64_t step = int64_t(gridDim.x) * blockDim.y;
   const float inv = 1.f / float(p.hidden);
   int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  Vec<T, kVec> x[kPer], dy[kPer];
-  load_row<T, kVec, kPer>(p.x, p.x_pitch, r, p.rows, p.hidden, x);
-  load_row<T, kVec, kPer>(p.dy, p.dy_pitch, r, p.rows, p.hidden, dy);
+  using Stream = RowStream<T, kVec, kPer>;
+  constexpr int kAhead = Stream::kShared ? kStages : 1;
+  Stream x(p.x, p.x_pitch, p.rows, p.hidden, smem_u32(rows_smem), 0, 2);
+  Stream dy(p.dy, p.dy_pitch, p.rows, p.hidden, smem_u32(rows_smem), 1, 2);
+  for (int i = 0; i < kAhead; ++i) {
+    x.request(r + i * step, i);
+    dy.request(r + i * step, i);
+    stream_commit();
+  }
   float mean = r < p.rows ? __ldg(p.mean + r) : 0.f, rstd = r < p.rows ? __ldg(p.rstd + r) : 0.f;
   Pair w[kPairs], dw[kPairs] = {}, db[kPairs] = {};
   load_params<T, kVec, kPer>(p.weight, p.params_fp32, p.hidden, 1.f, w);
   for (int64_t first = int64_t(blockIdx.x) * blockDim.y; first < p.rows; first += step, r += step) {
     Pair h[kPairs], g[kPairs];
-    take_apart<T, kVec, kPer>(x, h);
-    take_apart<T, kVec, kPer>(dy, g);
+    if (Stream::kShared) stream_wait();
+    x.take(stage, h);
+    dy.take(stage, g);
+    x.request(r + kAhead * step, stage);
+    dy.request(r + kAhead * step, stage);
+    stream_commit();
+    stage = stage + 1 == kAhead ? 0 : stage + 1;
     const Pair m2 = pair_of(-mean, -mean), r2 = pair_of(rstd, rstd);
     const bool here = r < p.rows;
     const bool more = r + step < p.rows;
-    load_row<T, kVec, kPer>(p.x, p.x_pitch, r + step, p.rows, p.hidden, x);
-    load_row<T, kVec, kPer>(p.dy, p.dy_pitch, r + step, p.rows, p.hidden, dy);
     mean = more ? __ldg(p.mean + r + step) : 0.f;
     rstd = more ? __ldg(p.rstd + r + step) : 0.f;
     Pair sg = 0, sgh = 0;
@@ -453,8 +570,8 @@ struct Plan {
 struct Shape {
   int per, most, threads_per_sm;
 };
-constexpr Shape kForwardVec[] = {{1, 512, 1024}, {2, 512, 1024}, {4, 512, 512}};
-constexpr Shape kForwardVecFew[] = {{1, 1024, 1024}, {2, 1024, 1024}, {4, 512, 512}};
+constexpr Shape kForwardVec[] = {{2, 64, 1024}, {4, 256, 512}, {4, 512, 512}};
+constexpr Shape kForwardVecFew[] = {{1, 1024, 1024}, {4, 512, 512}};
 constexpr Shape kForwardOne[] = {{4, 256, 1024}, {16, 1024, 1024}};
 constexpr Shape kForwardOneFew[] = {{4, 1024, 1024}, {16, 1024, 1024}};
 constexpr Shape kBackwardVec[] = {{1, 512, 1024}, {2, 512, 512}};
@@ -510,25 +627,44 @@ Plan make_plan(bool backward, int elem_bytes, bool aligned, int64_t rows, int64_
   return l;
 }
 
+using KernelFn = void (*)(const NormArgs);
 template <typename T>
-void launch_forward(const NormArgs& a, const Plan& l, cudaStream_t s) {
+KernelFn forward_kernel(const Plan& l) {
   constexpr int kV = 16 / sizeof(T);
-  if (l.vec == 0) norm_long_kernel<T><<<l.blocks, l.block, 0, s>>>(a);
-  else if (l.vec == 1 && l.per == 4) norm_kernel<T, 1, 4, 1024><<<l.blocks, l.block, 0, s>>>(a);
-  else if (l.vec == 1) norm_kernel<T, 1, 16, 1024><<<l.blocks, l.block, 0, s>>>(a);
-  else if (l.per == 1) norm_kernel<T, kV, 1, 1024><<<l.blocks, l.block, 0, s>>>(a);
-  else if (l.per == 2) norm_kernel<T, kV, 2, 1024><<<l.blocks, l.block, 0, s>>>(a);
-  else norm_kernel<T, kV, 4, 512><<<l.blocks, l.block, 0, s>>>(a);
+  if (l.vec == 0) return norm_long_kernel<T>;
+  if (l.vec == 1) return l.per == 4 ? norm_kernel<T, 1, 4, 1024, 1> : norm_kernel<T, 1, 16, 1024, 1>;
+  if (l.per == 1) return norm_kernel<T, kV, 1, 1024, 1>;
+  return l.per == 2 ? norm_kernel<T, kV, 2, 256, 4> : norm_kernel<T, kV, 4, 512, 1>;
 }
 template <typename T>
-void launch_backward(const NormArgs& a, const Plan& l, cudaStream_t s) {
+KernelFn backward_kernel(const Plan& l) {
   constexpr int kV = 16 / sizeof(T);
-  if (l.vec == 0) norm_grad_long_kernel<T><<<l.blocks, l.block, 0, s>>>(a);
-  else if (l.vec == 1 && l.per == 4) norm_grad_kernel<T, 1, 4, 1024><<<l.blocks, l.block, 0, s>>>(a);
-  else if (l.vec == 1) norm_grad_kernel<T, 1, 16, 512><<<l.blocks, l.block, 0, s>>>(a);
-  else if (l.per == 1) norm_grad_kernel<T, kV, 1, 1024><<<l.blocks, l.block, 0, s>>>(a);
-  else if (l.per == 2) norm_grad_kernel<T, kV, 2, 512><<<l.blocks, l.block, 0, s>>>(a);
-  else if constexpr (sizeof(T) == 4) norm_grad_kernel<T, kV, 4, 512><<<l.blocks, l.block, 0, s>>>(a);
+  if (l.vec == 0) return norm_grad_long_kernel<T>;
+  if (l.vec == 1) return l.per == 4 ? norm_grad_kernel<T, 1, 4, 1024> : norm_grad_kernel<T, 1, 16, 512>;
+  if (l.per == 1) return norm_grad_kernel<T, kV, 1, 1024>;
+  if constexpr (sizeof(T) == 4)
+    if (l.per == 4) return norm_grad_kernel<T, kV, 4, 512>;
+  return norm_grad_kernel<T, kV, 2, 512>;
+}
+
+int launch(bool backward, int precision, const NormArgs& a, const Plan& l, int device, cudaStream_t stream) {
+  const int type = precision == MB200_PRECISION_FP32 ? 0 : precision == MB200_PRECISION_FP16 ? 1 : 2;
+  const KernelFn kernel = type == 0   ? (backward ? backward_kernel<float>(l) : forward_kernel<float>(l))
+                          : type == 1 ? (backward ? backward_kernel<__half>(l) : forward_kernel<__half>(l))
+                                      : (backward ? backward_kernel<__nv_bfloat16>(l) : forward_kernel<__nv_bfloat16>(l));
+  const size_t smem = l.vec > 1 ? size_t(kStages) * l.block.x * l.block.y * l.per * 16 * (backward ? 2 : 1) : 0;
+  if (smem > 40 * 1024) {  // with the static share past the 48 KiB that need no asking
+    // the most any plan takes, once per device and kernel; a second thread that sets it again does no harm
+    static std::atomic<bool> configured[kMaxDevices][2][3][5];
+    std::atomic<bool>* done = device >= 0 && device < kMaxDevices ? &configured[device][backward][type][l.per] : nullptr;
+    if (!done || !done->load(std::memory_order_acquire)) {
+      MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024));
+      if (done) done->store(true, std::memory_order_release);
+    }
+  }
+  kernel<<<l.blocks, l.block, smem, stream>>>(a);
+  MB200_CHECK_CUDA(cudaGetLastError());
+  return kOk;
 }
 
 // Whether every row of every tensor starts on a 16-byte boundary.
@@ -580,11 +716,7 @@ int mb200_layer_norm(int precision, const void* x, int64_t x_pitch, int64_t rows
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int size = precision == MB200_PRECISION_FP32 ? 4 : 2;
   const Plan l = make_plan(false, size, rows_aligned(a, size), rows, hidden, device);
-  if (precision == MB200_PRECISION_FP32) launch_forward<float>(a, l, s);
-  else if (precision == MB200_PRECISION_FP16) launch_forward<__half>(a, l, s);
-  else launch_forward<__nv_bfloat16>(a, l, s);
-  MB200_CHECK_CUDA(cudaGetLastError());
-  return kOk;
+  return launch(false, precision, a, l, device, s);
 }
 
 int64_t mb200_layer_norm_backward_workspace_bytes(int64_t rows, int64_t hidden, int device) {
@@ -635,10 +767,7 @@ int mb200_layer_norm_backward(int precision, const void* dy, int64_t dy_pitch, c
                   (long long)workspace_bytes, (long long)need);
     a.sums = reinterpret_cast<float*>(workspace);
   }
-  if (precision == MB200_PRECISION_FP32) launch_backward<float>(a, l, s);
-  else if (precision == MB200_PRECISION_FP16) launch_backward<__half>(a, l, s);
-  else launch_backward<__nv_bfloat16>(a, l, s);
-  MB200_CHECK_CUDA(cudaGetLastError());
+  if ((rc = launch(true, precision, a, l, device, s))) return rc;
   if (a.sums) {
     norm_param_grad_kernel<<<unsigned((2 * hidden + 31) / 32), 256, 0, s>>>(a.sums, l.parts, hidden, dweight, dbias);
     MB200_CHECK_CUDA(cudaGetLastError());
