@@ -9,7 +9,7 @@
 #include <atomic>
 
 #include "../../include/moe_bench_b200.h"
-#include "layer.cuh"
+#include "linear.cuh"
 
 namespace mb200 {
 
@@ -534,24 +534,26 @@ __global__ void __launch_bounds__(kLongThreads) norm_grad_long_kernel(const Norm
   }
 }
 
-// dweight and dbias: the parts added in a fixed order, 32 columns x 8 lanes per block.
-__global__ void __launch_bounds__(256) norm_param_grad_kernel(const float* sums, int parts, int64_t hidden, float* dweight,
-                                                              float* dbias) {
-  __shared__ float lanes[8][32];
+// Parts added in a fixed order, 32 columns x 32 lanes per block: lane k takes parts k, k + 32, ..., then the lanes in order.
+constexpr int kSumLanes = 32;
+__global__ void __launch_bounds__(32 * kSumLanes) column_sums_kernel(const float* parts, int count, int64_t columns, float* out,
+                                                                     int64_t first, float* rest) {
+  __shared__ float lanes[kSumLanes][33];
   const int c = threadIdx.x & 31, lane = threadIdx.x >> 5;
   const int64_t i = int64_t(blockIdx.x) * 32 + c;
   float s = 0.f;
-  if (i < 2 * hidden)
-#pragma unroll 8
-    for (int b = lane; b < parts; b += 8) s += sums[int64_t(b) * 2 * hidden + i];
+  if (i < columns)
+#pragma unroll 4
+    for (int k = lane; k < count; k += kSumLanes) s += parts[k * columns + i];
   lanes[lane][c] = s;
   __syncthreads();
-  if (lane != 0 || i >= 2 * hidden) return;
-  for (int k = 1; k < 8; ++k) s += lanes[k][c];
-  if (i < hidden) {
-    if (dweight) dweight[i] = s;
-  } else if (dbias) {
-    dbias[i - hidden] = s;
+  s = warp_sum(lanes[c][lane]);  // this warp's column, one lane's sum per thread
+  const int64_t at = int64_t(blockIdx.x) * 32 + lane;
+  if (c != 0 || at >= columns) return;
+  if (at < first) {
+    if (out) out[at] = s;
+  } else if (rest) {
+    rest[at - first] = s;
   }
 }
 
@@ -686,6 +688,12 @@ int check_norm(int precision, int64_t rows, int64_t hidden, const char* what) {
 
 }  // namespace
 
+int launch_column_sums(const float* parts, int count, int64_t columns, float* out, int64_t first, float* rest, cudaStream_t stream) {
+  column_sums_kernel<<<unsigned((columns + 31) / 32), 32 * kSumLanes, 0, stream>>>(parts, count, columns, out, first, rest);
+  MB200_CHECK_CUDA(cudaGetLastError());
+  return kOk;
+}
+
 }  // namespace mb200
 
 using namespace mb200;
@@ -768,10 +776,7 @@ int mb200_layer_norm_backward(int precision, const void* dy, int64_t dy_pitch, c
     a.sums = reinterpret_cast<float*>(workspace);
   }
   if ((rc = launch(true, precision, a, l, device, s))) return rc;
-  if (a.sums) {
-    norm_param_grad_kernel<<<unsigned((2 * hidden + 31) / 32), 256, 0, s>>>(a.sums, l.parts, hidden, dweight, dbias);
-    MB200_CHECK_CUDA(cudaGetLastError());
-  }
+  if (a.sums) return launch_column_sums(a.sums, l.parts, 2 * hidden, dweight, hidden, dbias, s);
   return kOk;
 }
 

@@ -187,6 +187,11 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int m, int64_t row, i
     if (row + i * step < last) store4(e.out, e.out_fp32, e.fp16, m, row + i * step, f, z + 4 * i, vec);
 }
 
+// layer_norm.cu
+// out[i] = sum over k of parts[k][i], i < columns, in a fixed order; what lies from `first` on goes to `rest` instead.
+// Either may be null: its columns are left out.
+int launch_column_sums(const float* parts, int count, int64_t columns, float* out, int64_t first, float* rest, cudaStream_t stream);
+
 // products.cu
 // Bytes of workspace that launch_product wants for a dense product (one group), 0 where its sums are not split.
 int64_t product_workspace_bytes(ProductKind kind, int rows, int m, int n, int k, int device);
