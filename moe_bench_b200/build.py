@@ -21,7 +21,7 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ_DIR = os.path.join(PKG, "build")
 LIB_PATH = os.path.join(PKG, "libmoe_bench_b200.so")
 SOURCES = ["api.cu", "route_align.cu", "rows.cu", "grouped_gemm.cu", "grouped_gemm_fp8.cu", "grouped_gemm_fp8_cols.cu", "peer.cu", "dist.cu",
-           "linear.cu", "products.cu", "layer_norm.cu"]
+           "linear.cu", "products.cu", "few_rows.cu", "layer_norm.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "--extended-lambda",

@@ -564,6 +564,11 @@ def _output(t: Optional[torch.Tensor], like: torch.Tensor, shape, dtype, name: s
     return t
 
 
+def _dense_like(t: torch.Tensor, dtype) -> torch.Tensor:
+    """A new dense tensor of t's shape; of a dense t it costs two thirds of what naming the shape does."""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
 def _scratch(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
     if nbytes < 0:
         raise MB200Error(load().mb200_last_error().decode())
@@ -635,8 +640,8 @@ def linear_backward(dy, x, w, slope=None, dw_dtype=None, want_dx: bool = True, w
     if slope is not None:
         _output(slope, x, (rows, n), x.dtype, "slope")
     dw_dtype = _dw_type(w, dw_dtype)
-    dx = x.new_empty((rows, k)) if want_dx else None
-    dw = w.new_empty((n, k), dtype=dw_dtype) if want_dw else None
+    dx = _dense_like(x, x.dtype) if want_dx else None
+    dw = _dense_like(w, dw_dtype) if want_dw else None
     db = x.new_empty(n, dtype=torch.float32) if want_db else None
     lib, dev = load(), x.get_device()
     ws = _scratch(lib.mb200_linear_backward_workspace_bytes(rows, n, k, dev), x)
@@ -691,8 +696,10 @@ def grouped_linear_backward(dy, x, w, offsets, dw_dtype=None, dx_out=None, want_
     rows = x.shape[0]
     xp, dp = _pitch(x, x, (rows, k), "x"), _pitch(dy, x, (rows, n), "dy")
     dw_dtype = _dw_type(w, dw_dtype)
-    dx = _output(dx_out, x, (rows, k), x.dtype, "dx_out") if want_dx else None
-    dw = w.new_empty((e, n, k), dtype=dw_dtype) if want_dw else None
+    dx = None
+    if want_dx:
+        dx = _dense_like(x, x.dtype) if dx_out is None else _output(dx_out, x, (rows, k), x.dtype, "dx_out")
+    dw = _dense_like(w, dw_dtype) if want_dw else None
     lib, dev = load(), x.get_device()
     copied = dp % 8 or dy.data_ptr() % 16
     ws = _scratch(lib.mb200_grouped_linear_backward_workspace_bytes(rows, n), x) if copied else None
@@ -738,8 +745,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
             return layer_norm(x, weight, bias, eps, out)
     precision, rows, h, fp32 = _norm_operands(x, weight, bias, "layer_norm")
     xp = _pitch(x, x, (rows, h), "x")
-    y = _output(out, x, (rows, h), x.dtype, "out")
-    mean, rstd = x.new_empty((2, rows), dtype=torch.float32).unbind()
+    y = _dense_like(x, x.dtype) if out is None else _output(out, x, (rows, h), x.dtype, "out")
+    mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
     dev = x.get_device()
     rc = load().mb200_layer_norm(precision, x.data_ptr(), xp, rows, h, _ptr(weight), _ptr(bias), fp32, eps, y.data_ptr(),
                                  mean.data_ptr(), rstd.data_ptr(), dev, _raw_stream(dev))
@@ -757,7 +764,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, want_dx: bool = True, wa
     xp, dp = _pitch(x, x, (rows, h), "x"), _pitch(dy, x, (rows, h), "dy")
     for t, what in ((mean, "mean"), (rstd, "rstd")):
         _vector(t, x, rows, what, (torch.float32,))
-    dx = x.new_empty((rows, h)) if want_dx else None
+    dx = _dense_like(x, x.dtype) if want_dx else None
     dweight = x.new_empty(h, dtype=torch.float32) if want_dweight else None
     dbias = x.new_empty(h, dtype=torch.float32) if want_dbias else None
     lib, dev = load(), x.get_device()

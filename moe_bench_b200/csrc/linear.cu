@@ -237,7 +237,7 @@ extern "C" {
 
 int64_t mb200_linear_workspace_bytes(int64_t rows, int n, int k, int device) {
   if (check_sizes(rows, n, k, "linear_workspace_bytes")) return -1;
-  return product_workspace_bytes(kForward, int(rows), n, 0, k, device);
+  return rows <= kFewRows ? 0 : product_workspace_bytes(kForward, int(rows), n, 0, k, device);
 }
 
 int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, const void* w, int64_t w_pitch, int n,
@@ -270,6 +270,7 @@ int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, co
   p.epi.residual_pitch = residual_pitch;
   p.epi.slope = slope;
   p.epi.act = activation;
+  if (rows <= kFewRows) return launch_few_rows(p, device, as_stream(stream));
   return launch_product(kForward, p, workspace, workspace_bytes, device, as_stream(stream));
 }
 

@@ -187,10 +187,20 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int m, int64_t row, i
     if (row + i * step < last) store4(e.out, e.out_fp32, e.fp16, m, row + i * step, f, z + 4 * i, vec);
 }
 
+// Whether the epilogue can access four neighbouring features of every tensor at once.
+inline int epilogue_vec(const Epilogue& e, int m) {
+  auto at = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
+  return m % 4 == 0 && at(e.out, e.out_fp32 ? 16 : 8) && at(e.slope, 8) && (!e.residual || (at(e.residual, 8) && e.residual_pitch % 4 == 0));
+}
+
 // layer_norm.cu
 // out[i] = sum over k of parts[k][i], i < columns, in a fixed order; what lies from `first` on goes to `rest` instead.
 // Either may be null: its columns are left out.
 int launch_column_sums(const float* parts, int count, int64_t columns, float* out, int64_t first, float* rest, cudaStream_t stream);
+
+// few_rows.cu: the dense forward product of at most kFewRows rows
+constexpr int kFewRows = 16;
+int launch_few_rows(const ProductArgs& args, int device, cudaStream_t stream);
 
 // products.cu
 // Bytes of workspace that launch_product wants for a dense product (one group), 0 where its sums are not split.

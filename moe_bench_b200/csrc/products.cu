@@ -569,8 +569,7 @@ int launch_product(ProductKind kind, const ProductArgs& args, void* workspace, i
   MB200_REQUIRE(tiles < (int64_t(1) << 30), kUnsupportedShape, "product: %lld tiles do not fit 32-bit tile numbers",
                 (long long)tiles);
   const Epilogue& e = args.epi;
-  s.vec = args.m % 4 == 0 && aligned_to(e.out, e.out_fp32 ? 16 : 8) && (!e.slope || aligned_to(e.slope, 8)) &&
-          (!e.residual || (aligned_to(e.residual, 8) && e.residual_pitch % 4 == 0));
+  s.vec = epilogue_vec(e, args.m);
 
   const bool finish = e.bias || e.act || e.residual || e.slope;
   s.vec8 = !finish && !e.out_fp32 && s.splits == 1 && args.m % 8 == 0 && aligned_to(e.out, 16);
