@@ -362,11 +362,9 @@ int mb200_read_status(const void* workspace, int32_t* status_out, void* stream);
  * if out_fp32.  slope: NULL, or [rows, n] in the precision's type that receives act'(z), the
  * one thing of the forward that the backward call below needs besides x and w.  y may be the
  * residual's buffer (same type and pitch n). */
-int64_t mb200_linear_workspace_bytes(int64_t rows, int n, int k, int device);
 int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, const void* w, int64_t w_pitch,
                  int n, int k, const void* bias, int bias_fp32, int activation, const void* residual,
-                 int64_t residual_pitch, void* y, int out_fp32, void* slope, void* workspace,
-                 int64_t workspace_bytes, int device, void* stream);
+                 int64_t residual_pitch, void* y, int out_fp32, void* slope, int device, void* stream);
 
 /* Gradients of mb200_linear (the residual's is dy itself).  dz = dy * slope (slope NULL: dz = dy):
  * dx = dz . w [rows, k]; dw = dz^T . x [n, k], fp32 if dw_fp32; db = sum of dz over the rows, fp32

@@ -85,11 +85,10 @@ SIGNATURES = {
     "mb200_set_fp8_scale_format": (c_i32, [c_i32]),
     "mb200_set_comm_only": (c_i32, [c_i32]),
     "mb200_read_status": (c_i32, [c_vp, c_vp, c_vp]),
-    "mb200_linear_workspace_bytes": (c_i64, [c_i64, c_i32, c_i32, c_i32]),
     "mb200_linear": (
         c_i32,
         [c_i32, c_vp, c_i64, c_i64, c_vp, c_i64, c_i32, c_i32, c_vp, c_i32, c_i32, c_vp, c_i64, c_vp, c_i32, c_vp,
-         c_vp, c_i64, c_i32, c_vp],
+         c_i32, c_vp],
     ),
     "mb200_linear_backward_workspace_bytes": (c_i64, [c_i64, c_i32, c_i32, c_i32]),
     "mb200_linear_backward": (
@@ -604,12 +603,11 @@ def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, o
         raise MB200Error(f"linear: output of {out_dtype} for operands of {x.dtype}")
     y = _output(out, x, (rows, n), out_dtype, "out")
     slope = x.new_empty((rows, n)) if want_slope else None
-    lib, dev = load(), x.get_device()
-    ws = _scratch(lib.mb200_linear_workspace_bytes(rows, n, k, dev), x)
-    rc = lib.mb200_linear(
+    dev = x.get_device()
+    rc = load().mb200_linear(
         precision, x.data_ptr(), xp, rows, w.data_ptr(), wp, n, k, _ptr(bias), bias is not None and bias.dtype == torch.float32,
-        ACTIVATIONS[activation], _ptr(residual), rp, y.data_ptr(), out_dtype == torch.float32, _ptr(slope), _ptr(ws),
-        0 if ws is None else ws.numel(), dev, _raw_stream(dev),
+        ACTIVATIONS[activation], _ptr(residual), rp, y.data_ptr(), out_dtype == torch.float32, _ptr(slope), dev,
+        _raw_stream(dev),
     )
     _check(rc, "linear")
     return (y, slope) if want_slope else y

@@ -133,14 +133,6 @@ GradLayout grad_layout(int64_t rows, int n, int device) {
   return l;
 }
 
-// Bytes behind dz: the column sums, and after them, in the same place, the parts of one product's split sums.
-int64_t split_bytes(int64_t rows, int n, int k, int device, bool dx, bool dw, int64_t sum_bytes) {
-  int64_t b = sum_bytes;
-  if (rows > 0 && dx) b = std::max(b, product_workspace_bytes(kInputGrad, int(rows), k, 0, n, device));
-  if (rows > 0 && dw) b = std::max(b, product_workspace_bytes(kWeightGrad, int(rows), k, n, 0, device));
-  return b;
-}
-
 int check_precision(int precision, const char* what) {
   MB200_REQUIRE(precision == MB200_PRECISION_BF16 || precision == MB200_PRECISION_FP16, kInvalidArgument,
                 "%s: precision %d (bf16 or fp16)", what, precision);
@@ -235,15 +227,9 @@ using namespace mb200;
 
 extern "C" {
 
-int64_t mb200_linear_workspace_bytes(int64_t rows, int n, int k, int device) {
-  if (check_sizes(rows, n, k, "linear_workspace_bytes")) return -1;
-  return rows <= kFewRows ? 0 : product_workspace_bytes(kForward, int(rows), n, 0, k, device);
-}
-
 int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, const void* w, int64_t w_pitch, int n,
                  int k, const void* bias, int bias_fp32, int activation, const void* residual, int64_t residual_pitch,
-                 void* y, int out_fp32, void* slope, void* workspace, int64_t workspace_bytes, int device,
-                 void* stream) {
+                 void* y, int out_fp32, void* slope, int device, void* stream) {
   const char* what = "linear";
   int rc;
   if ((rc = check_precision(precision, what)) || (rc = check_sizes(rows, n, k, what))) return rc;
@@ -271,13 +257,13 @@ int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, co
   p.epi.slope = slope;
   p.epi.act = activation;
   if (rows <= kFewRows) return launch_few_rows(p, device, as_stream(stream));
-  return launch_product(kForward, p, workspace, workspace_bytes, device, as_stream(stream));
+  return launch_product(kForward, p, device, as_stream(stream));
 }
 
 int64_t mb200_linear_backward_workspace_bytes(int64_t rows, int n, int k, int device) {
   if (check_sizes(rows, n, k, "linear_backward_workspace_bytes")) return -1;
   const GradLayout l = grad_layout(rows, n, device);
-  return l.dz_bytes + split_bytes(rows, n, k, device, true, true, l.sum_bytes);
+  return l.dz_bytes + l.sum_bytes;
 }
 
 int mb200_linear_backward(int precision, const void* dy, int dy_fp32, int64_t dy_pitch, const void* slope, const void* x,
@@ -300,13 +286,9 @@ int mb200_linear_backward(int precision, const void* dy, int dy_fp32, int64_t dy
   MB200_REQUIRE(dy != nullptr, kInvalidArgument, "linear_backward: dy is null");
   if (dx && (rc = check_operand(w, w_pitch, k, what, "w"))) return rc;
   if (dw && (rc = check_operand(x, x_pitch, k, what, "x"))) return rc;
-  const void* given = dy;
   if ((rc = prepare_output_grad(what, dy, dy_fp32, dy_pitch, slope, rows, n, fp16, dx || dw, db, workspace,
                                 workspace_bytes, device, s)))
     return rc;
-  const int64_t dz_bytes = dy == given ? 0 : grad_layout(rows, n, device).dz_bytes;
-  void* parts = workspace ? reinterpret_cast<char*>(workspace) + dz_bytes : nullptr;
-  const int64_t part_bytes = workspace_bytes - dz_bytes;
   ProductArgs p{};
   p.b = dy;
   p.b_pitch = dy_pitch;
@@ -319,13 +301,13 @@ int mb200_linear_backward(int precision, const void* dy, int dy_fp32, int64_t dy
     p.a = w;
     p.a_pitch = w_pitch;
     p.epi = plain_output(dx, 0, fp16);
-    if ((rc = launch_product(kInputGrad, p, parts, part_bytes, device, s))) return rc;
+    if ((rc = launch_product(kInputGrad, p, device, s))) return rc;
   }
   if (dw) {
     p.a = x;
     p.a_pitch = x_pitch;
     p.epi = plain_output(dw, dw_fp32 != 0, fp16);
-    if ((rc = launch_product(kWeightGrad, p, parts, part_bytes, device, s))) return rc;
+    if ((rc = launch_product(kWeightGrad, p, device, s))) return rc;
   }
   return kOk;
 }
@@ -353,7 +335,7 @@ int mb200_grouped_linear(int precision, const void* x, int64_t x_pitch, int64_t 
   p.m = n;
   p.k = k;
   p.epi = plain_output(y, 0, precision == MB200_PRECISION_FP16);
-  return launch_product(kForward, p, nullptr, 0, device, as_stream(stream));
+  return launch_product(kForward, p, device, as_stream(stream));
 }
 
 int64_t mb200_grouped_linear_backward_workspace_bytes(int64_t rows, int n) {
@@ -396,13 +378,13 @@ int mb200_grouped_linear_backward(int precision, const void* dy, int64_t dy_pitc
     p.a_pitch = w_pitch;
     p.a_group = w_expert_pitch;
     p.epi = plain_output(dx, 0, fp16);
-    if ((rc = launch_product(kInputGrad, p, nullptr, 0, device, s))) return rc;
+    if ((rc = launch_product(kInputGrad, p, device, s))) return rc;
   }
   if (dw) {
     p.a = x;
     p.a_pitch = x_pitch;
     p.epi = plain_output(dw, dw_fp32 != 0, fp16);
-    if ((rc = launch_product(kWeightGrad, p, nullptr, 0, device, s))) return rc;
+    if ((rc = launch_product(kWeightGrad, p, device, s))) return rc;
   }
   return kOk;
 }

@@ -203,11 +203,8 @@ constexpr int kFewRows = 16;
 int launch_few_rows(const ProductArgs& args, int device, cudaStream_t stream);
 
 // products.cu
-// Bytes of workspace that launch_product wants for a dense product (one group), 0 where its sums are not split.
-int64_t product_workspace_bytes(ProductKind kind, int rows, int m, int n, int k, int device);
 // status word of the products on the current device
 int product_status(int* status_out, int clear, cudaStream_t stream);
-int launch_product(ProductKind kind, const ProductArgs& args, void* workspace, int64_t workspace_bytes, int device,
-                   cudaStream_t stream);
+int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaStream_t stream);
 
 }  // namespace mb200

@@ -19,6 +19,7 @@
 // output rows at a time go through a 2 KiB block of shared memory that turns them round, still in fp32, and leave
 // through the epilogue as 64 contiguous bytes per output row.  Every wait is bounded.
 
+#include <algorithm>
 #include <atomic>
 
 #include "linear.cuh"
@@ -67,9 +68,7 @@ struct Maps {
 struct TileShape {
   int f_tiles;      // feature blocks
   int row_blocks;   // weight gradient: blocks of output rows per group
-  int splits;       // parts of every sum, each with a tile of its own
-  float* partial;   // [splits][output rows][partial_pitch] where splits > 1
-  int64_t partial_rows, partial_pitch;
+  int splits;       // pairs of CTAs that share a tile, each with a part of its sums; they form a cluster
   int vec;          // the epilogue may access four features at once
   int vec8;         // nothing but sums rounded to 16 bits, eight features at once
 };
@@ -84,18 +83,12 @@ struct Tile {
   int cols, valid;    // output rows computed, and stored
   int c_begin;        // weight gradient: first row of the segment
   int depth;          // terms of the whole sum
-  int step0, step1;   // steps of this part
-  int split;
+  int step0, step1;   // steps of this pair's part
 };
 
 template <int kKind>
-__device__ __forceinline__ Tile locate(int tile, const ProductArgs& p, const TileShape& s, const SmemTail* t) {
+__device__ __forceinline__ Tile locate(int tile, int part, const ProductArgs& p, const TileShape& s, const SmemTail* t) {
   Tile r;
-  r.split = 0;
-  if (s.splits > 1) {
-    r.split = tile % s.splits;
-    tile /= s.splits;
-  }
   int blocks, local;
   if (kKind == kWeightGrad) {
     blocks = s.row_blocks;
@@ -145,14 +138,107 @@ __device__ __forceinline__ Tile locate(int tile, const ProductArgs& p, const Til
     r.depth = p.k;
   }
   const int steps = (r.depth + kStep - 1) / kStep;
-  r.step0 = s.splits > 1 ? int(int64_t(steps) * r.split / s.splits) : 0;
-  r.step1 = s.splits > 1 ? int(int64_t(steps) * (r.split + 1) / s.splits) : steps;
+  r.step0 = s.splits > 1 ? int(int64_t(steps) * part / s.splits) : 0;
+  r.step1 = s.splits > 1 ? int(int64_t(steps) * (part + 1) / s.splits) : steps;
   return r;
+}
+
+// 32 features x 16 output rows, a feature per lane, turned round: 4 neighbouring features of rows (lane / 8) + 4 i per thread.
+__device__ __forceinline__ void turn_chunk(float* block, const uint32_t (&v)[16], bool summed, float (&z)[16]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) block[i * 32 + lane] = summed ? __uint_as_float(v[i]) : 0.f;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(z + 4 * i) =
+      *reinterpret_cast<const float4*>(block + ((lane >> 3) + 4 * i) * 32 + 4 * (lane & 7));
+  __syncwarp();
+}
+
+// Such a chunk through the epilogue.
+template <bool kFinish>
+__device__ __forceinline__ void emit(const ProductArgs& p, const TileShape& shape, const Tile& c, int chunk, int f, float (&z)[16],
+                                     const Bias4& bias, const Residual4<4>& res) {
+  const int64_t row = c.out_row + chunk * 16 + ((threadIdx.x & 31) >> 3), last = c.out_row + c.valid;
+  if (kFinish) {
+    finish4<4>(p.epi, p.m, row, 4, last, f, z, bias, res, shape.vec);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (row + 4 * i < last) store4(p.epi.out, p.epi.out_fp32, p.epi.fp16, p.m, row + 4 * i, f, z + 4 * i, shape.vec);
+  }
+}
+
+// The pairs of a cluster have a part of the same tile's sums each, in tensor memory.  Pair k finishes the chunks
+// k, k + splits, ...: it gets the other pairs' parts of them pushed into its ring, which nothing uses any more, and adds them in
+// the pairs' order.  Called by all threads of the cluster; a cluster has one tile at most.
+template <int kKind, bool kFinish>
+__device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape& shape, SmemTail* t, uint32_t ring, uint32_t tmem,
+                                           int worker, int part, uint32_t cta, int total_tiles, WaitCtx& ctx) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quarter = warp & 3, group = (warp - kFirstEpilogueWarp) >> 2;
+  const bool mine = warp >= kFirstEpilogueWarp && worker < total_tiles;
+  const int splits = shape.splits;
+  Tile c{};
+  bool ok = false;
+  if (mine) {
+    c = locate<kKind>(worker, part, p, shape, t);
+    ok = mbar_wait(smem_u32(&t->acc_full[0]), 0, ctx, 26);
+    tc_fence_after();
+  }
+  __syncwarp();
+  cluster_sync();  // every pair's products have read their stages
+  const bool summed = c.step1 > c.step0;
+  const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
+  const int chunks = (c.valid + 15) >> 4;
+  // block of [16 rows][32 features] for chunk k of pair `from`, in the ring of the pair that finishes it
+  auto block_of = [&](int k, int from) { return uint32_t(((k / splits * splits + from) * 4 + quarter) * 2048); };
+  if (ok) {
+    for (int k = group; k < chunks; k += 2) {
+      if (k % splits == part) continue;
+      uint32_t v[16];
+      tmem_ld16(lanes + k * 16, v);
+      tmem_ld_wait();
+      const uint32_t to = map_to_cta(ring + block_of(k, part), uint32_t(k % splits) * 2 + (cta & 1)) + lane * 4;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + i * 128), "r"(summed ? v[i] : 0u) : "memory");
+    }
+  }
+  __syncwarp();
+  cluster_sync();
+  if (!ok) return;
+  const int f = c.f0 + int(cta & 1) * 128 + quarter * 32 + 4 * (lane & 7);
+  Bias4 bias{};
+  if (kFinish) bias = load_bias4(p.epi, p.m, f);
+  for (int k = part + group * splits; k < chunks; k += 2 * splits) {
+    Residual4<4> res{};
+    if (kFinish) res = load_residual4<4>(p.epi, p.m, c.out_row + k * 16 + (lane >> 3), 4, c.out_row + c.valid, f, shape.vec);
+    uint32_t v[16];
+    tmem_ld16(lanes + k * 16, v);
+    tmem_ld_wait();
+    float own[16], z[16] = {};
+    turn_chunk(t->turn[warp - kFirstEpilogueWarp], v, summed, own);
+    for (int from = 0; from < splits; ++from) {
+      const uint32_t at = ring + block_of(k, from) + (lane >> 3) * 128 + (lane & 7) * 16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float4 q;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w) : "r"(at + i * 512) : "memory");
+        const float* o = own + 4 * i;
+        z[4 * i] += from == part ? o[0] : q.x;
+        z[4 * i + 1] += from == part ? o[1] : q.y;
+        z[4 * i + 2] += from == part ? o[2] : q.z;
+        z[4 * i + 3] += from == part ? o[3] : q.w;
+      }
+    }
+    emit<kFinish>(p, shape, c, k, f, z, bias, res);
+  }
 }
 
 // kFinish: the output is more than the rounded sum (bias, activation, residual or slope)
 template <int kKind, bool kFinish>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const TileShape shape) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -160,8 +246,11 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
   const uint32_t ring = raw_addr + pad;
   SmemTail* t = reinterpret_cast<SmemTail*>(smem_raw + pad + kRingBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
-  const int worker = blockIdx.x >> 1, workers = gridDim.x >> 1;
+  // a cluster is `splits` pairs of CTAs: this CTA's place in its pair, the pair's place, the pair's first CTA
+  const uint32_t cta = cluster_rank(), rank = cta & 1, first_cta = cta & ~1u;
+  const int part = int(cta >> 1);
+  const int worker = int(blockIdx.x) / (2 * shape.splits), workers = int(gridDim.x) / (2 * shape.splits);
+  const uint16_t pair_mask = uint16_t(3u << first_cta);
 
   if (threadIdx.x == 0) {
     prefetch_tmap(&maps.a);
@@ -220,7 +309,6 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     total_tiles = t->blocks[p.groups] * shape.f_tiles;
     half_rows = min(128, (t->max_len + 31) / 32 * 16);
   }
-  total_tiles *= shape.splits;
   const int stage_bytes = kABytes + max(half_rows, 16) * 128;
   const int stages = min(kMaxStages, int(kRingBytes) / stage_bytes);
   tc_fence_before();
@@ -229,6 +317,9 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
   const uint32_t tmem = t->tmem_base;
   WaitCtx ctx{&t->abort_flag, g_status, wait_limit_ns(g_status)};
 
+  const int quarter = warp & 3;                              // tensor-memory lanes 32*quarter .. +31 of an epilogue warp
+  const int first_chunk = (warp - kFirstEpilogueWarp) >> 2;  // its chunks of 16 output rows: every other one
+
   if (warp == 0) {
     // ---------------- loads ----------------
     if (lane < kBoxes) prefetch_tmap(&maps.b[lane]);
@@ -236,7 +327,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     uint32_t phase = 0;
     bool ok = true;
     for (int tile = worker; ok && tile < total_tiles; tile += workers) {
-      const Tile c = locate<kKind>(tile, p, shape, t);
+      const Tile c = locate<kKind>(tile, part, p, shape, t);
       const int half = c.cols >> 1;
       const int f = c.f0 + int(rank) * 128, j = c.b_row + int(rank) * half;
       const uint32_t bytes = kABytes + half * 128;
@@ -247,7 +338,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
         if (elect_one()) {
           const bool tail = ragged && kb == c.depth / kStep;
           const uint32_t own_bar = smem_u32(tail ? &t->raw[stage] : &t->full[stage]);
-          const uint32_t bar = tail ? map_to_cta(own_bar, rank) : map_to_cta(own_bar, 0);
+          const uint32_t bar = map_to_cta(own_bar, tail ? cta : first_cta);
           if (tail) {
             mbar_expect_tx(own_bar, bytes);
           } else if (rank == 0) {
@@ -289,7 +380,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     bool ok = true;
     const uint32_t fmt = p.epi.fp16 ? 0u : 1u;
     for (int tile = worker; rank == 0 && ok && tile < total_tiles; tile += workers, ++it) {
-      const Tile c = locate<kKind>(tile, p, shape, t);
+      const Tile c = locate<kKind>(tile, part, p, shape, t);
       const uint32_t buf = it & 1, use = it >> 1;
       ok = mbar_wait_cluster(smem_u32(&t->acc_empty[buf]), (use & 1) ^ 1, ctx, 22);
       if (!ok) break;
@@ -312,12 +403,12 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
           for (int k = 0; k < 4; ++k)
             if (k < parts)
               umma_h16_pair(d, a_desc + kAStep * k, b_desc + kBStep * k, idesc, kb > c.step0 || k > 0);
-          tc_commit_pair(smem_u32(&t->empty[stage]));
+          tc_commit_pair(smem_u32(&t->empty[stage]), pair_mask);
         }
         __syncwarp();
         if (++stage == stages) { stage = 0; phase ^= 1; }
       }
-      if (ok && elect_one()) tc_commit_pair(smem_u32(&t->acc_full[buf]));
+      if (ok && elect_one()) tc_commit_pair(smem_u32(&t->acc_full[buf]), pair_mask);
       __syncwarp();
     }
   } else if (warp == 2) {
@@ -326,7 +417,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     uint32_t phases = 0;  // parity of raw[stage], one bit each
     bool ok = true;
     for (int tile = worker; kKind == kWeightGrad && ok && tile < total_tiles; tile += workers) {
-      const Tile c = locate<kKind>(tile, p, shape, t);
+      const Tile c = locate<kKind>(tile, part, p, shape, t);
       const int last = c.depth / kStep;
       if (c.depth % kStep != 0 && last >= c.step0 && last < c.step1) {
         const int at = (stage + last - c.step0) % stages;
@@ -344,62 +435,29 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + box * 8192 + r * 128), "r"(0) : "memory");
         fence_proxy_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&t->full[at]), 0));
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&t->full[at]), first_cta));
         __syncwarp();
       }
       stage = (stage + c.step1 - c.step0) % stages;
     }
-  } else if (warp >= kFirstEpilogueWarp) {
+  } else if (warp >= kFirstEpilogueWarp && shape.splits == 1) {
     // ---------------- epilogue: each warp on 32 features ----------------
-    const int quarter = warp & 3;                                   // tensor-memory lanes 32*quarter .. +31
-    const int first_chunk = (warp - kFirstEpilogueWarp) >> 2;       // chunks of 16 output rows, every other one
     float* turn = t->turn[warp - kFirstEpilogueWarp];
     uint32_t it = 0;
     for (int tile = worker; tile < total_tiles; tile += workers, ++it) {
-      const Tile c = locate<kKind>(tile, p, shape, t);
+      const Tile c = locate<kKind>(tile, part, p, shape, t);
       const uint32_t buf = it & 1, use = it >> 1;
       const int f = c.f0 + int(rank) * 128 + quarter * 32 + 4 * (lane & 7);
       Bias4 bias{};
-      if (kFinish && shape.splits == 1) bias = load_bias4(p.epi, p.m, f);
+      if (kFinish) bias = load_bias4(p.epi, p.m, f);
       const bool summed = c.step1 > c.step0;
       const uint32_t lanes = tmem + buf * 256 + (uint32_t(quarter * 32) << 16);
       const int chunks = (c.valid + 15) >> 4;
-      const int64_t last = c.out_row + c.valid;
-      auto emit = [&](int chunk, const uint32_t (&v)[16], const Residual4<4>& res) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) turn[i * 32 + lane] = summed ? __uint_as_float(v[i]) : 0.f;
-        __syncwarp();
-        float z[16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 s = *reinterpret_cast<const float4*>(turn + ((lane >> 3) + 4 * i) * 32 + 4 * (lane & 7));
-          z[4 * i] = s.x;
-          z[4 * i + 1] = s.y;
-          z[4 * i + 2] = s.z;
-          z[4 * i + 3] = s.w;
-        }
-        __syncwarp();
-        const int64_t row = c.out_row + chunk * 16 + (lane >> 3);
-        if (shape.splits > 1) {
-          if (f < p.m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (row + 4 * i < last)
-                *reinterpret_cast<float4*>(shape.partial + (c.split * shape.partial_rows + row + 4 * i) * shape.partial_pitch + f) =
-                    make_float4(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
-        } else if (kFinish) {
-          finish4<4>(p.epi, p.m, row, 4, last, f, z, bias, res, shape.vec);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (row + 4 * i < last) store4(p.epi.out, p.epi.out_fp32, p.epi.fp16, p.m, row + 4 * i, f, z + 4 * i, shape.vec);
-        }
-      };
       bool released = false;
       auto release = [&]() {  // this warp's share is in registers: the accumulator may be overwritten
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&t->acc_empty[buf]), 0));
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&t->acc_empty[buf]), first_cta));
         released = true;
       };
       if (!kFinish && shape.vec8 && summed) {
@@ -449,8 +507,8 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
       } else {
         // a chunk's share of the residual is requested one chunk ahead
         Residual4<4> res{};
-        const bool with_residual = kFinish && shape.splits == 1;
-        if (with_residual && first_chunk < chunks)
+        const int64_t last = c.out_row + c.valid;
+        if (kFinish && first_chunk < chunks)
           res = load_residual4<4>(p.epi, p.m, c.out_row + first_chunk * 16 + (lane >> 3), 4, last, f, shape.vec);
         if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
         tc_fence_after();
@@ -458,17 +516,21 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
           uint32_t v[16];
           tmem_ld16(lanes + k * 16, v);
           Residual4<4> next{};
-          if (with_residual && k + 2 < chunks)
+          if (kFinish && k + 2 < chunks)
             next = load_residual4<4>(p.epi, p.m, c.out_row + (k + 2) * 16 + (lane >> 3), 4, last, f, shape.vec);
           tmem_ld_wait();
           if (k + 2 >= chunks) release();
-          emit(k, v, res);
+          float z[16];
+          turn_chunk(turn, v, summed, z);
+          emit<kFinish>(p, shape, c, k, f, z, bias, res);
           res = next;
         }
       }
       if (!released) release();
     }
   }
+
+  if (shape.splits > 1) join_parts<kKind, kFinish>(p, shape, t, ring, tmem, worker, part, cta, total_tiles, ctx);
 
   // ---------------- teardown ----------------
   __syncwarp();
@@ -482,38 +544,15 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
   if (warp == 3) tmem_dealloc_pair(tmem, kTmemCols);
 }
 
-// Split sums: the parts added in order, then the epilogue.
-__global__ void __launch_bounds__(256) join_kernel(const ProductArgs p, const TileShape s) {
-  const int64_t vecs = s.partial_pitch / 4, total = s.partial_rows * vecs;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-    const int64_t row = i / vecs;
-    const int f = int(i - row * vecs) * 4;
-    float z[4] = {0.f, 0.f, 0.f, 0.f};
-    const float* part = s.partial + row * s.partial_pitch + f;
-    for (int k = 0; k < s.splits; ++k) {
-      const float4 v = *reinterpret_cast<const float4*>(part + k * s.partial_rows * s.partial_pitch);
-      z[0] += v.x;
-      z[1] += v.y;
-      z[2] += v.z;
-      z[3] += v.w;
-    }
-    finish4<1>(p.epi, p.m, row, 1, row + 1, f, z, load_bias4(p.epi, p.m, f),
-               load_residual4<1>(p.epi, p.m, row, 1, row + 1, f, s.vec), s.vec);
-  }
-}
-
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// A dense product of few tiles leaves most pairs idle: its sums are split, at least four steps to a part.
-int split_count(ProductKind kind, int64_t rows, int m, int n, int k, int device) {
-  const int pairs = device_sm_count(device) / 2;
-  const int64_t tiles = ceil_div(m, kTileFeatures) * ceil_div(kind == kWeightGrad ? n : rows, kTileRows);
-  const int64_t steps = ceil_div(kind == kWeightGrad ? rows : k, kStep);
-  int64_t s = tiles > 0 ? pairs / tiles : 1;
-  if (s > steps / 4) s = steps / 4;
-  return int(s < 1 ? 1 : s);
+// Few tiles leave most pairs of CTAs idle: up to four share a tile then, at least four steps to a part.  `tiles`: as many
+// as there can be.
+int split_count(int64_t tiles, int64_t steps, int sms) {
+  int s = 4;
+  while (s > 1 && (tiles * 2 * s > sms || steps < 4 * s)) s /= 2;
+  return s;
 }
-int64_t partial_pitch(int m) { return ceil_div(m, 4) * 4; }
 
 // Tiled view of 16-bit elements: c0 side by side, c1 `pitch` elements apart, c2 `group` elements apart.
 int make_map(CUtensorMap* map, const void* base, int64_t c0, int64_t c1, int64_t c2, int64_t pitch, int64_t group,
@@ -533,11 +572,6 @@ KernelFn kernel_of(bool finish) {
 
 }  // namespace
 
-int64_t product_workspace_bytes(ProductKind kind, int rows, int m, int n, int k, int device) {
-  const int s = split_count(kind, rows, m, n, k, device);
-  return s > 1 ? s * int64_t(kind == kWeightGrad ? n : rows) * partial_pitch(m) * 4 : 0;
-}
-
 int product_status(int* status_out, int clear, cudaStream_t stream) {
   MB200_CHECK_CUDA(cudaStreamSynchronize(stream));
   MB200_CHECK_CUDA(cudaMemcpyFromSymbol(status_out, g_status, sizeof(int)));
@@ -546,33 +580,25 @@ int product_status(int* status_out, int clear, cudaStream_t stream) {
   return kOk;
 }
 
-int launch_product(ProductKind kind, const ProductArgs& args, void* workspace, int64_t workspace_bytes, int device,
-                   cudaStream_t stream) {
+int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaStream_t stream) {
   const int sms = device_sm_count(device);
   MB200_REQUIRE(sms > 1, kCudaError, "product: cannot read the SM count of device %d", device);
   const bool weight = kind == kWeightGrad;
   TileShape s{};
   s.f_tiles = int(ceil_div(args.m, kTileFeatures));
   s.row_blocks = weight ? int(ceil_div(args.n, kTileRows)) : 0;
-  s.splits = args.offsets ? 1 : split_count(kind, args.rows, args.m, args.n, args.k, device);
-  s.partial_rows = weight ? args.n : args.rows;
-  s.partial_pitch = partial_pitch(args.m);
-  if (s.splits > 1) {
-    const int64_t need = s.splits * s.partial_rows * s.partial_pitch * 4;
-    MB200_REQUIRE(workspace && aligned_to(workspace, 16), kInvalidArgument, "product: needs a 16-byte aligned workspace");
-    MB200_REQUIRE(workspace_bytes >= need, kWorkspaceTooSmall, "product: workspace %lld < %lld bytes",
-                  (long long)workspace_bytes, (long long)need);
-    s.partial = reinterpret_cast<float*>(workspace);
-  }
-  const int64_t tiles = (weight ? int64_t(args.groups) * s.row_blocks : int64_t(args.rows) / kTileRows + args.groups) *
-                        s.f_tiles * s.splits;
+  // a segment's last block may be short: at most one more per segment than the rows fill
+  const int64_t blocks = weight ? int64_t(args.groups) * s.row_blocks
+                         : args.offsets ? int64_t(args.rows) / kTileRows + std::min(args.groups, args.rows)
+                                        : ceil_div(args.rows, kTileRows);
+  const int64_t tiles = blocks * s.f_tiles;
   MB200_REQUIRE(tiles < (int64_t(1) << 30), kUnsupportedShape, "product: %lld tiles do not fit 32-bit tile numbers",
                 (long long)tiles);
+  s.splits = split_count(tiles, ceil_div(weight ? args.rows / args.groups : args.k, kStep), sms);
   const Epilogue& e = args.epi;
   s.vec = epilogue_vec(e, args.m);
-
   const bool finish = e.bias || e.act || e.residual || e.slope;
-  s.vec8 = !finish && !e.out_fp32 && s.splits == 1 && args.m % 8 == 0 && aligned_to(e.out, 16);
+  s.vec8 = !finish && !e.out_fp32 && args.m % 8 == 0 && aligned_to(e.out, 16);
 
   Maps maps;
   int rc;
@@ -591,16 +617,22 @@ int launch_product(ProductKind kind, const ProductArgs& args, void* workspace, i
   static std::atomic<bool> configured[kMaxDevices][4];
   if (device < 0 || device >= kMaxDevices || !configured[device][variant].load(std::memory_order_acquire)) {
     MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)));
+    MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     if (device >= 0 && device < kMaxDevices) configured[device][variant].store(true, std::memory_order_release);
   }
-  const int64_t pairs = tiles < sms / 2 ? (tiles < 1 ? 1 : tiles) : sms / 2;
-  kernel<<<unsigned(2 * pairs), kThreads, kSmemBytes, stream>>>(maps, args, s);
-  MB200_CHECK_CUDA(cudaGetLastError());
-  if (s.splits > 1) {
-    const int64_t blocks = ceil_div(s.partial_rows * s.partial_pitch / 4, 256);
-    join_kernel<<<unsigned(blocks < 8 * sms ? blocks : 8 * sms), 256, 0, stream>>>(args, s);
-    MB200_CHECK_CUDA(cudaGetLastError());
-  }
+  const int64_t workers = std::min(tiles, int64_t(sms / 2));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(2 * s.splits);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(workers) * 2 * s.splits);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  MB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps, args, s));
   return kOk;
 }
 

@@ -21,11 +21,10 @@ P = 1 << 20  # an aligned address that no refused call touches
 
 
 def _linear(lib, **kw):
-    a = dict(precision=0, x=P, xp=64, rows=4, w=P, wp=64, n=5, k=64, bias=None, b32=0, act=0, res=None, rp=0, y=P, o32=0, slope=None,
-             ws=None, wsn=0)
+    a = dict(precision=0, x=P, xp=64, rows=4, w=P, wp=64, n=5, k=64, bias=None, b32=0, act=0, res=None, rp=0, y=P, o32=0, slope=None)
     a.update(kw)
     return lib.mb200_linear(a["precision"], a["x"], a["xp"], a["rows"], a["w"], a["wp"], a["n"], a["k"], a["bias"], a["b32"],
-                            a["act"], a["res"], a["rp"], a["y"], a["o32"], a["slope"], a["ws"], a["wsn"], 0, None)
+                            a["act"], a["res"], a["rp"], a["y"], a["o32"], a["slope"], 0, None)
 
 
 @pytest.mark.parametrize("change,words", [
@@ -102,7 +101,6 @@ def test_norm_refuses(lib):
 
 
 def test_workspace_queries_refuse_bad_sizes(lib):
-    assert lib.mb200_linear_workspace_bytes(4, 0, 64, 0) == -1
     assert lib.mb200_linear_backward_workspace_bytes(4, 8, 12, 0) == -1
     assert lib.mb200_grouped_linear_backward_workspace_bytes(-1, 8) == -1
     assert lib.mb200_layer_norm_backward_workspace_bytes(4, 0, 0) == -1
