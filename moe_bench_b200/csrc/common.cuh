@@ -396,6 +396,13 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uin
                "r"(c), "r"(d)
                : "memory");
 }
+// The way back: shared memory to the fragments, with the same addresses.
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+               : "r"(addr)
+               : "memory");
+}
 __device__ __forceinline__ uint32_t pack_h16x2(float lo, float hi, int fp16) {
   if (fp16) {
     const __half2 h = __floats2half2_rn(lo, hi);

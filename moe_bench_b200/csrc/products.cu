@@ -70,11 +70,10 @@ struct TileShape {
   int row_blocks;   // weight gradient: blocks of output rows per group
   int splits;       // pairs of CTAs that share a tile, each with a part of its sums; they form a cluster
   int vec;          // the epilogue may access four features at once
-  int vec8;         // nothing but sums rounded to 16 bits, eight features at once
+  int vec8;         // the output is of 16 bits, and every tensor takes eight features as one access
 };
 
-// first failure of a wait, wait limit in ms, 0, 0
-__device__ int g_status[4];
+__device__ int g_status[1];  // first failure of a wait
 
 struct Tile {
   int group, f0;
@@ -252,30 +251,45 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
   const int worker = int(blockIdx.x) / (2 * shape.splits), workers = int(gridDim.x) / (2 * shape.splits);
   const uint16_t pair_mask = uint16_t(3u << first_cta);
 
-  if (threadIdx.x == 0) {
-    prefetch_tmap(&maps.a);
-    for (int s = 0; s < kMaxStages; ++s) {
-      mbar_init(smem_u32(&t->full[s]), kKind == kWeightGrad ? 2 : 1);
-      mbar_init(smem_u32(&t->empty[s]), 1);
-      mbar_init(smem_u32(&t->raw[s]), 1);
+  if (warp == 0) {
+    if (lane < kMaxStages) {
+      mbar_init(smem_u32(&t->full[lane]), kKind == kWeightGrad ? 2 : 1);
+      mbar_init(smem_u32(&t->empty[lane]), 1);
+      mbar_init(smem_u32(&t->raw[lane]), 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(smem_u32(&t->acc_full[b]), 1);
-      mbar_init(smem_u32(&t->acc_empty[b]), 2 * kEpilogueWarps);
+    if (lane < 2) {
+      mbar_init(smem_u32(&t->acc_full[lane]), 1);
+      mbar_init(smem_u32(&t->acc_empty[lane]), 2 * kEpilogueWarps);
     }
-    t->abort_flag = 0;
-    t->max_len = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  } else if (warp == 1) {
+    if (lane == 0) {
+      prefetch_tmap(&maps.a);
+      t->abort_flag = 0;
+      t->max_len = 0;
+      if (p.offsets == nullptr) {
+        t->begin[0] = 0;
+        t->len[0] = p.rows;
+        t->blocks[0] = 0;
+        t->blocks[1] = (p.rows + kTileRows - 1) / kTileRows;
+      }
+    } else if (lane <= kBoxes) {
+      prefetch_tmap(&maps.b[lane - 1]);
+    }
+  } else if (warp == 3) {
+    tmem_alloc_pair(smem_u32(&t->tmem_base), kTmemCols);
   }
-  if (warp == 3) tmem_alloc_pair(smem_u32(&t->tmem_base), kTmemCols);
-  __syncthreads();
 
   int total_tiles;
   int half_rows = 128;  // rows of b that a CTA loads for a step at most
   if (kKind == kWeightGrad) {
     total_tiles = p.groups * shape.row_blocks * shape.f_tiles;
     if (p.n <= 128) half_rows = 64;
+  } else if (p.offsets == nullptr) {
+    total_tiles = (p.rows + kTileRows - 1) / kTileRows * shape.f_tiles;
+    half_rows = min(128, (p.rows + 31) / 32 * 16);
   } else {
+    __syncthreads();  // max_len is 0
     int longest = 0;
     for (int g = threadIdx.x; g < p.groups; g += kThreads) {
       int begin, end;
@@ -315,14 +329,13 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
   cluster_sync();  // both CTAs' barriers exist
   tc_fence_after();
   const uint32_t tmem = t->tmem_base;
-  WaitCtx ctx{&t->abort_flag, g_status, wait_limit_ns(g_status)};
+  WaitCtx ctx{&t->abort_flag, g_status, kDefaultWaitLimitNs};
 
   const int quarter = warp & 3;                              // tensor-memory lanes 32*quarter .. +31 of an epilogue warp
   const int first_chunk = (warp - kFirstEpilogueWarp) >> 2;  // its chunks of 16 output rows: every other one
 
   if (warp == 0) {
     // ---------------- loads ----------------
-    if (lane < kBoxes) prefetch_tmap(&maps.b[lane]);
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -460,15 +473,63 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
         if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&t->acc_empty[buf]), first_cta));
         released = true;
       };
-      if (!kFinish && shape.vec8 && summed) {
-        if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
-        tc_fence_after();
-        // 16-bit sums and nothing else: two chunks at a time, read as fragments of 8x8 matrices, rounded two output
-        // rows per instruction, transposed by stmatrix into 1 KiB each ([row][32 features], the 16-byte pieces of a
-        // row XOR-swizzled) and stored 8 features per thread
+      if (shape.vec8 && summed) {
+        // 16-bit outputs: two chunks at a time, read as fragments of 8x8 matrices (a lane has features 8m + lane / 4 of
+        // two neighbouring output rows), finished in that layout, rounded two rows per instruction, transposed by stmatrix
+        // into 1 KiB each ([row][32 features], the 16-byte pieces of a row XOR-swizzled) and stored 8 features per
+        // thread.  The residual comes in the same way backwards, a pair of chunks ahead.
         uint16_t* block = reinterpret_cast<uint16_t*>(turn);
         const uint32_t st_addr = smem_u32(block) + uint32_t(lane & 7) * 64 + (uint32_t(lane >> 3) ^ ((lane >> 1) & 3u)) * 16;
         const int f8 = c.f0 + int(rank) * 128 + quarter * 32 + (lane & 3) * 8;
+        // 16-byte piece i of this lane's four in a pair of chunks: its row and its place in `block`
+        auto row_of = [&](int k, int i) { return (k + 2 * (i >> 1)) * 16 + 8 * (i & 1) + (lane >> 2); };
+        auto place_of = [&](int i) {
+          const int piece = lane + 32 * (i & 1);
+          return reinterpret_cast<uint4*>(block + (i >> 1) * 512 + (piece >> 2) * 32 + ((piece & 3) ^ ((piece >> 3) & 3)) * 8);
+        };
+        uint4 res[4] = {};
+        auto request = [&](int k) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (row_of(k, i) < c.valid && f8 < p.m)
+              res[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.epi.residual) +
+                                                       (c.out_row + row_of(k, i)) * p.epi.residual_pitch + f8);
+        };
+        auto store = [&](void* out, int k) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 q = *place_of(i);
+            if (row_of(k, i) < c.valid && f8 < p.m)
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + (c.out_row + row_of(k, i)) * p.m + f8) = q;
+          }
+          __syncwarp();
+        };
+        // h[2m + r]: features 8m .., rows 8r .. of chunk u of the pair, of values in fragment order
+        auto place = [&](int u, const float (&z)[16]) {
+          uint32_t h[8];
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int i = (m >> 1) * 8 + r * 4 + (m & 1) * 2;
+              h[2 * m + r] = pack_h16x2(z[i], z[i + 1], p.epi.fp16);
+            }
+          stmatrix_x4_trans(st_addr + u * 1024, h[0], h[2], h[4], h[6]);
+          stmatrix_x4_trans(st_addr + u * 1024 + 8 * 64, h[1], h[3], h[5], h[7]);
+        };
+        float bias_m[4] = {};
+        if (kFinish) {
+          if (p.epi.bias)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              const int fm = f8 - (lane & 3) * 8 + 8 * m + (lane >> 2);
+              if (fm < p.m) bias_m[m] = p.epi.bias_fp32 ? __ldg(reinterpret_cast<const float*>(p.epi.bias) + fm) : load_h16(p.epi.bias, fm, p.epi.fp16);
+            }
+          if (p.epi.residual) request(first_chunk);
+        }
+        if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
+        tc_fence_after();
         for (int k = first_chunk; k < chunks; k += 4) {
           uint32_t v[2][16];
 #pragma unroll
@@ -479,30 +540,55 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
             }
           tmem_ld_wait();
           if (k + 4 >= chunks) release();
+          if (!kFinish) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint32_t h[8];  // h[2m + t]: features 8m .., rows 8t .. of the chunk
+            for (int u = 0; u < 2; ++u) {
+              float z[16];
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const int i = (m >> 1) * 8 + r * 4 + (m & 1) * 2;
-                h[2 * m + r] = pack_h16x2(__uint_as_float(v[u][i]), __uint_as_float(v[u][i + 1]), p.epi.fp16);
-              }
-            stmatrix_x4_trans(st_addr + u * 1024, h[0], h[2], h[4], h[6]);
-            stmatrix_x4_trans(st_addr + u * 1024 + 8 * 64, h[1], h[3], h[5], h[7]);
+              for (int i = 0; i < 16; ++i) z[i] = __uint_as_float(v[u][i]);
+              place(u, z);
+            }
+            store(p.epi.out, k);
+            continue;
           }
-          __syncwarp();
+          float z[2][16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int piece = lane + 32 * (i & 1);
-            const int row = (k + 2 * (i >> 1)) * 16 + (piece >> 2);
-            const uint4 q = *reinterpret_cast<const uint4*>(block + (i >> 1) * 512 + (piece >> 2) * 32 +
-                                                            ((piece & 3) ^ ((piece >> 3) & 3)) * 8);
-            if (row < c.valid && f8 < p.m)
-              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.epi.out) + (c.out_row + row) * p.m + f8) = q;
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) z[u][i] = __uint_as_float(v[u][i]) + bias_m[(i >> 3) * 2 + ((i >> 1) & 1)];
+          if (p.epi.slope) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              float slope[16];
+              activate<true>(p.epi.act, z[u], slope);
+              place(u, slope);
+            }
+            store(p.epi.slope, k);
+          } else if (p.epi.act) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              float slope[16];
+              activate<false>(p.epi.act, z[u], slope);
+            }
           }
-          __syncwarp();
+          if (p.epi.residual) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *place_of(i) = res[i];
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              uint32_t h[8];
+              ldmatrix_x4_trans(st_addr + u * 1024, h[0], h[2], h[4], h[6]);
+              ldmatrix_x4_trans(st_addr + u * 1024 + 8 * 64, h[1], h[3], h[5], h[7]);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) z[u][i] += load_h16(&h[((i >> 3) * 2 + ((i >> 1) & 1)) * 2 + ((i >> 2) & 1)], i & 1, p.epi.fp16);
+            }
+            if (k + 4 < chunks) request(k + 4);
+            __syncwarp();
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) place(u, z[u]);
+          store(p.epi.out, k);
         }
       } else {
         // a chunk's share of the residual is requested one chunk ahead
@@ -598,7 +684,8 @@ int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaSt
   const Epilogue& e = args.epi;
   s.vec = epilogue_vec(e, args.m);
   const bool finish = e.bias || e.act || e.residual || e.slope;
-  s.vec8 = !finish && !e.out_fp32 && args.m % 8 == 0 && aligned_to(e.out, 16);
+  s.vec8 = !e.out_fp32 && args.m % 8 == 0 && aligned_to(e.out, 16) && aligned_to(e.slope, 16) &&
+           (!e.residual || (aligned_to(e.residual, 16) && e.residual_pitch % 8 == 0));
 
   Maps maps;
   int rc;
