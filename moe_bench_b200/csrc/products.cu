@@ -632,11 +632,44 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Few tiles leave most pairs of CTAs idle: up to four share a tile then, at least four steps to a part.  `tiles`: as many
-// as there can be.
-int split_count(int64_t tiles, int64_t steps, int sms) {
-  int s = 4;
-  while (s > 1 && (tiles * 2 * s > sms || steps < 4 * s)) s /= 2;
+constexpr int kMaxSplits = 8;  // clusters of 16 CTAs
+
+cudaLaunchConfig_t cluster_config(int clusters, int splits, cudaStream_t stream, cudaLaunchAttribute* attr) {
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = unsigned(2 * splits);
+  attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(clusters) * 2 * splits);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// Clusters of `splits` pairs that run at the same time; it depends on how many SMs the parts of this GPU have (74, 33, 22,
+// 15, 11, 7, 7 and 7 on one B200).  Read once per device; a second thread that reads it again does no harm.
+int active_clusters(const void* kernel, int splits, int device) {
+  static std::atomic<int> cached[kMaxDevices][kMaxSplits + 1];
+  std::atomic<int>* slot = device >= 0 && device < kMaxDevices ? &cached[device][splits] : nullptr;
+  int n = slot ? slot->load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  cudaLaunchAttribute attr[1];
+  const cudaLaunchConfig_t cfg = cluster_config(1, splits, nullptr, attr);
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  if (slot && n > 0) slot->store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Few tiles leave most pairs of CTAs idle: up to eight share a tile then, as long as all clusters run at the same time and
+// each pair has four steps.  `tiles`: as many as there can be.
+int split_count(const void* kernel, int64_t tiles, int64_t steps, int device) {
+  int s = int(std::min(int64_t(kMaxSplits), std::max(steps / 4, int64_t(1))));
+  while (s > 1 && tiles > active_clusters(kernel, s, device)) --s;
   return s;
 }
 
@@ -680,7 +713,6 @@ int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaSt
   const int64_t tiles = blocks * s.f_tiles;
   MB200_REQUIRE(tiles < (int64_t(1) << 30), kUnsupportedShape, "product: %lld tiles do not fit 32-bit tile numbers",
                 (long long)tiles);
-  s.splits = split_count(tiles, ceil_div(weight ? args.rows / args.groups : args.k, kStep), sms);
   const Epilogue& e = args.epi;
   s.vec = epilogue_vec(e, args.m);
   const bool finish = e.bias || e.act || e.residual || e.slope;
@@ -707,18 +739,12 @@ int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaSt
     MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     if (device >= 0 && device < kMaxDevices) configured[device][variant].store(true, std::memory_order_release);
   }
-  const int64_t workers = std::min(tiles, int64_t(sms / 2));
+  // beyond half of the pairs nothing is split: the launch need not ask
+  s.splits = tiles * 2 > sms / 2
+                 ? 1
+                 : split_count(reinterpret_cast<const void*>(kernel), tiles, ceil_div(weight ? args.rows / args.groups : args.k, kStep), device);
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = unsigned(2 * s.splits);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(workers) * 2 * s.splits);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmemBytes;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  const cudaLaunchConfig_t cfg = cluster_config(int(std::min(tiles, int64_t(sms / 2))), s.splits, stream, attr);
   MB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps, args, s));
   return kOk;
 }
