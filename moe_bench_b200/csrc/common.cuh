@@ -466,12 +466,11 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// mbar_wait for a barrier that the other CTA's threads arrive on.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, WaitCtx& ctx, int where) {
+// mbar_wait_lane for a barrier that the other CTA's threads arrive on.
+__device__ __forceinline__ bool mbar_wait_cluster_lane(uint32_t bar, uint32_t parity, WaitCtx& ctx, int where) {
   uint32_t spins = 0;
   WaitClock clock;
-  bool done = false, expired = false;
-  while (!done && !expired) {
+  while (true) {
     uint32_t ok;
     asm volatile(
         "{\n\t"
@@ -482,16 +481,29 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
-    done = ok != 0;
-    if (!done && (++spins & 0x3FF) == 0) {
-      if (*ctx.abort_flag) expired = true;
-      else if (clock.expired(ctx)) {
+    if (ok) return true;
+    if ((++spins & 0x3FF) == 0) {
+      if (*ctx.abort_flag) return false;
+      if (clock.expired(ctx)) {
         wait_give_up(ctx, where);
-        expired = true;
+        return false;
       }
     }
   }
-  return __all_sync(0xffffffffu, done);
+}
+// One poll of such a barrier, for a wait that comes later.
+__device__ __forceinline__ uint32_t mbar_peek_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
 }
 // 3-D tiled load into this CTA's shared memory that completes on a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap, int c0, int c1, int c2, uint32_t cluster_bar) {
