@@ -554,9 +554,7 @@ def _vector(t: Optional[torch.Tensor], like: torch.Tensor, n: int, name: str, dt
                          f"{like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _output(t: Optional[torch.Tensor], like: torch.Tensor, shape, dtype, name: str) -> torch.Tensor:
-    if t is None:
-        return like.new_empty(shape, dtype=dtype)
+def _output(t: torch.Tensor, like: torch.Tensor, shape, dtype, name: str) -> torch.Tensor:
     if t.dtype != dtype or t.get_device() != like.get_device() or t.shape != shape or not t.is_contiguous():
         raise MB200Error(f"{name}: need a contiguous tensor of {dtype} {tuple(shape)} on {like.device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
@@ -574,9 +572,9 @@ def _scratch(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
     return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
-def _elsewhere(x: torch.Tensor) -> bool:
-    """Whether x lives on another GPU than the current one: the call is then made again with x's device current."""
-    return x.is_cuda and x.get_device() != _current_device()
+def _elsewhere(device: int) -> bool:
+    """Whether that device (negative: the CPU) is another GPU than the current one: the call is then made again with it current."""
+    return device >= 0 and device != _current_device()
 
 
 def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, out_dtype=None, want_slope: bool = False):
@@ -585,28 +583,30 @@ def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, o
     Rows may be further apart than they are long (a multiple of 8 elements); ``k`` is a multiple of 8, ``n`` is free.
     ``out`` may be the residual itself.  With ``want_slope`` also returns ``act'(x @ w.T + bias)`` in x's type, which
     ``linear_backward`` takes."""
-    if _elsewhere(x):
-        with torch.cuda.device(x.device):
+    dev = x.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return linear(x, w, bias, activation, residual, out, out_dtype, want_slope)
     precision = _h16(x, "x")
     if x.dim() != 2 or w.dim() != 2:
         raise MB200Error(f"linear: need matrices, got x {tuple(x.shape)} and w {tuple(w.shape)}")
     rows, k = x.shape
     n = w.shape[0]
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise MB200Error(f"activation {activation!r}: expected one of {sorted(ACTIVATIONS)}")
-    xp, wp = _pitch(x, x, (rows, k), "x"), _pitch(w, x, (n, k), "w")
+    xp = k if rows > 1 and x.is_contiguous() else _pitch(x, x, (rows, k), "x")
+    wp = _pitch(w, x, (n, k), "w")
     _vector(bias, x, n, "bias", (x.dtype, torch.float32))
     rp = _pitch(residual, x, (rows, n), "residual") if residual is not None else 0
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in (x.dtype, torch.float32):
         raise MB200Error(f"linear: output of {out_dtype} for operands of {x.dtype}")
-    y = _output(out, x, (rows, n), out_dtype, "out")
+    y = x.new_empty((rows, n), dtype=out_dtype) if out is None else _output(out, x, (rows, n), out_dtype, "out")
     slope = x.new_empty((rows, n)) if want_slope else None
-    dev = x.get_device()
     rc = load().mb200_linear(
         precision, x.data_ptr(), xp, rows, w.data_ptr(), wp, n, k, _ptr(bias), bias is not None and bias.dtype == torch.float32,
-        ACTIVATIONS[activation], _ptr(residual), rp, y.data_ptr(), out_dtype == torch.float32, _ptr(slope), dev,
+        act, _ptr(residual), rp, y.data_ptr(), out_dtype == torch.float32, _ptr(slope), dev,
         _raw_stream(dev),
     )
     _check(rc, "linear")
@@ -624,8 +624,9 @@ def linear_backward(dy, x, w, slope=None, dw_dtype=None, want_dx: bool = True, w
     """Gradients ``(dx, dw, db)`` of ``linear`` (None where not wanted; the residual's gradient is ``dy``).  ``slope``: what
     ``linear(..., want_slope=True)`` returned, None for no activation.  ``dy`` may be fp32 for bf16 operands.  ``dy * slope``
     is rounded to x's type once, for the products; ``db`` is its fp32 sum before that; ``dw`` has w's type, or fp32."""
-    if _elsewhere(x):
-        with torch.cuda.device(x.device):
+    dev = x.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return linear_backward(dy, x, w, slope, dw_dtype, want_dx, want_dw, want_db)
     precision = _h16(x, "x")
     if x.dim() != 2 or w.dim() != 2:
@@ -641,8 +642,9 @@ def linear_backward(dy, x, w, slope=None, dw_dtype=None, want_dx: bool = True, w
     dx = _dense_like(x, x.dtype) if want_dx else None
     dw = _dense_like(w, dw_dtype) if want_dw else None
     db = x.new_empty(n, dtype=torch.float32) if want_db else None
-    lib, dev = load(), x.get_device()
-    ws = _scratch(lib.mb200_linear_backward_workspace_bytes(rows, n, k, dev), x)
+    lib = load()
+    copied = slope is not None or dp % 8 or dy.dtype == torch.float32 or dy.data_ptr() % 16
+    ws = _scratch(lib.mb200_linear_backward_workspace_bytes(rows, n, 1 if copied else 0, dev), x)
     rc = lib.mb200_linear_backward(
         precision, dy.data_ptr(), dy.dtype == torch.float32, dp, _ptr(slope), x.data_ptr(), xp, rows, w.data_ptr(), wp, n, k,
         _ptr(dx), _ptr(dw), dw_dtype == torch.float32, _ptr(db), _ptr(ws), 0 if ws is None else ws.numel(), dev, _raw_stream(dev),
@@ -668,15 +670,15 @@ def grouped_linear(x, w, offsets, out=None):
     """``x[r] @ w[e].T`` for the rows of segment e = ``offsets[e] .. offsets[e + 1] - 1``, of any length: x [rows, k] and
     w [experts, n, k] of bf16 or fp16, offsets [experts + 1] int32 on x's device (``align(..., pad_rows=1)`` returns them as
     ``mtile_prefix``).  Rows outside the segments are left as they are in ``out``, undefined in a tensor made here."""
-    if _elsewhere(x):
-        with torch.cuda.device(x.device):
+    dev = x.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return grouped_linear(x, w, offsets, out)
     precision = _h16(x, "x")
     e, n, k, wp, ep = _expert_weight(w, x, offsets)
     rows = x.shape[0]
     xp = _pitch(x, x, (rows, k), "x")
-    y = _output(out, x, (rows, n), x.dtype, "out")
-    dev = x.get_device()
+    y = x.new_empty((rows, n)) if out is None else _output(out, x, (rows, n), x.dtype, "out")
     rc = load().mb200_grouped_linear(precision, x.data_ptr(), xp, rows, w.data_ptr(), wp, ep, offsets.data_ptr(), e, n, k,
                                      y.data_ptr(), dev, _raw_stream(dev))
     _check(rc, "grouped_linear")
@@ -686,8 +688,9 @@ def grouped_linear(x, w, offsets, out=None):
 def grouped_linear_backward(dy, x, w, offsets, dw_dtype=None, dx_out=None, want_dx: bool = True, want_dw: bool = True):
     """Gradients ``(dx, dw)`` of ``grouped_linear`` (None where not wanted).  Rows outside the segments have no part in
     ``dw`` and are left as they are in ``dx_out``; an expert without rows gets a zero gradient.  ``dw`` has w's type, or fp32."""
-    if _elsewhere(x):
-        with torch.cuda.device(x.device):
+    dev = x.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return grouped_linear_backward(dy, x, w, offsets, dw_dtype, dx_out, want_dx, want_dw)
     precision = _h16(x, "x")
     e, n, k, wp, ep = _expert_weight(w, x, offsets)
@@ -698,7 +701,7 @@ def grouped_linear_backward(dy, x, w, offsets, dw_dtype=None, dx_out=None, want_
     if want_dx:
         dx = _dense_like(x, x.dtype) if dx_out is None else _output(dx_out, x, (rows, k), x.dtype, "dx_out")
     dw = _dense_like(w, dw_dtype) if want_dw else None
-    lib, dev = load(), x.get_device()
+    lib = load()
     copied = dp % 8 or dy.data_ptr() % 16
     ws = _scratch(lib.mb200_grouped_linear_backward_workspace_bytes(rows, n), x) if copied else None
     rc = lib.mb200_grouped_linear_backward(
@@ -738,14 +741,14 @@ def _norm_operands(x, weight, bias, name: str):
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     """Layer norm of the rows of ``x [rows, hidden]`` (bf16, fp16 or fp32; rows may be any distance apart): returns
     ``(y, mean, rstd)``, the last two in fp32 for ``layer_norm_backward``.  weight and bias have x's type or fp32."""
-    if _elsewhere(x):
-        with torch.cuda.device(x.device):
+    dev = x.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return layer_norm(x, weight, bias, eps, out)
     precision, rows, h, fp32 = _norm_operands(x, weight, bias, "layer_norm")
     xp = _pitch(x, x, (rows, h), "x")
     y = _dense_like(x, x.dtype) if out is None else _output(out, x, (rows, h), x.dtype, "out")
     mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
-    dev = x.get_device()
     rc = load().mb200_layer_norm(precision, x.data_ptr(), xp, rows, h, _ptr(weight), _ptr(bias), fp32, eps, y.data_ptr(),
                                  mean.data_ptr(), rstd.data_ptr(), dev, _raw_stream(dev))
     _check(rc, "layer_norm")
@@ -755,8 +758,9 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
 def layer_norm_backward(dy, x, mean, rstd, weight=None, want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
     """Gradients ``(dx, dweight, dbias)`` of ``layer_norm`` (None where not wanted); the last two are fp32 sums over the rows,
     in a fixed order."""
-    if _elsewhere(x):
-        with torch.cuda.device(x.device):
+    dev = x.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return layer_norm_backward(dy, x, mean, rstd, weight, want_dx, want_dweight, want_dbias)
     precision, rows, h, fp32 = _norm_operands(x, weight, None, "layer_norm_backward")
     xp, dp = _pitch(x, x, (rows, h), "x"), _pitch(dy, x, (rows, h), "dy")
@@ -765,7 +769,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, want_dx: bool = True, wa
     dx = _dense_like(x, x.dtype) if want_dx else None
     dweight = x.new_empty(h, dtype=torch.float32) if want_dweight else None
     dbias = x.new_empty(h, dtype=torch.float32) if want_dbias else None
-    lib, dev = load(), x.get_device()
+    lib = load()
     ws = None
     if want_dweight or want_dbias:
         ws = _scratch(lib.mb200_layer_norm_backward_workspace_bytes(rows, h, dev), x)

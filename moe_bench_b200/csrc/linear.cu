@@ -260,10 +260,10 @@ int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, co
   return launch_product(kForward, p, device, as_stream(stream));
 }
 
-int64_t mb200_linear_backward_workspace_bytes(int64_t rows, int n, int k, int device) {
-  if (check_sizes(rows, n, k, "linear_backward_workspace_bytes")) return -1;
+int64_t mb200_linear_backward_workspace_bytes(int64_t rows, int n, int copies_dy, int device) {
+  if (check_sizes(rows, n, 8, "linear_backward_workspace_bytes")) return -1;
   const GradLayout l = grad_layout(rows, n, device);
-  return l.dz_bytes + l.sum_bytes;
+  return (copies_dy ? l.dz_bytes : 0) + l.sum_bytes;
 }
 
 int mb200_linear_backward(int precision, const void* dy, int dy_fp32, int64_t dy_pitch, const void* slope, const void* x,

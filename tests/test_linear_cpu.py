@@ -101,7 +101,7 @@ def test_norm_refuses(lib):
 
 
 def test_workspace_queries_refuse_bad_sizes(lib):
-    assert lib.mb200_linear_backward_workspace_bytes(4, 8, 12, 0) == -1
+    assert lib.mb200_linear_backward_workspace_bytes(4, 0, 1, 0) == -1
     assert lib.mb200_grouped_linear_backward_workspace_bytes(-1, 8) == -1
     assert lib.mb200_layer_norm_backward_workspace_bytes(4, 0, 0) == -1
 
