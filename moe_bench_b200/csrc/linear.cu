@@ -297,19 +297,8 @@ int mb200_linear_backward(int precision, const void* dy, int dy_fp32, int64_t dy
   p.m = k;
   p.n = n;
   p.k = n;
-  if (dx) {
-    p.a = w;
-    p.a_pitch = w_pitch;
-    p.epi = plain_output(dx, 0, fp16);
-    if ((rc = launch_product(kInputGrad, p, device, s))) return rc;
-  }
-  if (dw) {
-    p.a = x;
-    p.a_pitch = x_pitch;
-    p.epi = plain_output(dw, dw_fp32 != 0, fp16);
-    if ((rc = launch_product(kWeightGrad, p, device, s))) return rc;
-  }
-  return kOk;
+  p.epi = plain_output(nullptr, 0, fp16);
+  return launch_gradients(p, dx, dw, dw_fp32 != 0, w, w_pitch, 0, x, x_pitch, device, s);
 }
 
 int mb200_grouped_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, const void* w, int64_t w_pitch,
@@ -373,20 +362,8 @@ int mb200_grouped_linear_backward(int precision, const void* dy, int64_t dy_pitc
   p.m = k;
   p.n = n;
   p.k = n;
-  if (dx) {
-    p.a = w;
-    p.a_pitch = w_pitch;
-    p.a_group = w_expert_pitch;
-    p.epi = plain_output(dx, 0, fp16);
-    if ((rc = launch_product(kInputGrad, p, device, s))) return rc;
-  }
-  if (dw) {
-    p.a = x;
-    p.a_pitch = x_pitch;
-    p.epi = plain_output(dw, dw_fp32 != 0, fp16);
-    if ((rc = launch_product(kWeightGrad, p, device, s))) return rc;
-  }
-  return kOk;
+  p.epi = plain_output(nullptr, 0, fp16);
+  return launch_gradients(p, dx, dw, dw_fp32 != 0, w, w_pitch, w_expert_pitch, x, x_pitch, device, s);
 }
 
 int mb200_linear_status(int32_t* status_out, int clear, void* stream) {

@@ -26,7 +26,8 @@ struct Epilogue {
 //   forward      out[row][f] = sum_k  w[g][f][k] x[row][k]         rows of segment g
 //   input grad   out[row][f] = sum_n  w[g][n][f] dz[row][n]        rows of segment g
 //   weight grad  out[g*n + j][f] = sum_row x[row][f] dz[row][j]    rows of segment g
-enum ProductKind : int { kForward = 0, kInputGrad = 1, kWeightGrad = 2 };
+// Both gradients can be one launch: they share dz and their features.
+enum ProductKind : int { kForward = 0, kInputGrad = 1, kWeightGrad = 2, kBothGrads = 3 };
 struct ProductArgs {
   const void* a;            // feature side: w, w, x
   const void* b;            // row side: x, dz, dz
@@ -38,6 +39,11 @@ struct ProductArgs {
   int n;                    // weight grad: output rows per group
   int k;                    // forward, input grad: length of the sum
   Epilogue epi;
+  // both gradients: x and the weight gradient, beside a = w and epi.out = the input gradient
+  const void* a2;
+  int64_t a2_pitch;
+  void* out2;
+  int out2_fp32;
 };
 
 // Segment g of the rows, cut to [0, rows] whatever the offsets hold.
@@ -206,5 +212,8 @@ int launch_few_rows(const ProductArgs& args, int device, cudaStream_t stream);
 // status word of the products on the current device
 int product_status(int* status_out, int clear, cudaStream_t stream);
 int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaStream_t stream);
+// The gradients of a forward product that are wanted (dx or dw may be null): `args` says the rest, b = dz among it.
+int launch_gradients(const ProductArgs& args, void* dx, void* dw, int dw_fp32, const void* w, int64_t w_pitch, int64_t w_group,
+                     const void* x, int64_t x_pitch, int device, cudaStream_t stream);
 
 }  // namespace mb200

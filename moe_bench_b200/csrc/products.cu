@@ -62,6 +62,7 @@ static_assert(kRingBytes >= 6 * (kABytes + 128 * 128), "full tiles want six stag
 
 struct Maps {
   CUtensorMap a;
+  CUtensorMap a2;  // both gradients: x
   CUtensorMap b[kBoxes];
 };
 
@@ -70,12 +71,14 @@ struct TileShape {
   int row_blocks;   // weight gradient: blocks of output rows per group
   int splits;       // pairs of CTAs that share a tile, each with a part of its sums; they form a cluster
   int vec;          // the epilogue may access four features at once
+  int vec2, vec8_2; // the same two for the weight gradient where both gradients are computed
   int vec8;         // the output is of 16 bits, and every tensor takes eight features as one access
 };
 
 __device__ int g_status[1];  // first failure of a wait
 
 struct Tile {
+  int weight;         // a tile of the weight gradient
   int group, f0;
   int64_t out_row;    // first output row
   int b_row;          // its row coordinate in b (weight gradient: its column)
@@ -86,8 +89,9 @@ struct Tile {
 };
 
 template <int kKind>
-__device__ __forceinline__ Tile locate(int tile, int part, const ProductArgs& p, const TileShape& s, const SmemTail* t) {
+__device__ __forceinline__ Tile locate_tile(int tile, int part, const ProductArgs& p, const TileShape& s, const SmemTail* t) {
   Tile r;
+  r.weight = kKind == kWeightGrad;
   int blocks, local;
   if (kKind == kWeightGrad) {
     blocks = s.row_blocks;
@@ -142,6 +146,14 @@ __device__ __forceinline__ Tile locate(int tile, int part, const ProductArgs& p,
   return r;
 }
 
+// Both gradients: the input gradient's tiles, then the weight gradient's, so that only one wave of tiles is the last.
+template <int kKind>
+__device__ __forceinline__ Tile locate(int tile, int first_tiles, int part, const ProductArgs& p, const TileShape& s, const SmemTail* t) {
+  if constexpr (kKind != kBothGrads) return locate_tile<kKind>(tile, part, p, s, t);
+  else if (tile < first_tiles) return locate_tile<kInputGrad>(tile, part, p, s, t);
+  else return locate_tile<kWeightGrad>(tile - first_tiles, part, p, s, t);
+}
+
 // 32 features x 16 output rows, a feature per lane, turned round: 4 neighbouring features of rows (lane / 8) + 4 i per thread.
 __device__ __forceinline__ void turn_chunk(float* block, const uint32_t (&v)[16], bool summed, float (&z)[16]) {
   const int lane = threadIdx.x & 31;
@@ -155,16 +167,23 @@ __device__ __forceinline__ void turn_chunk(float* block, const uint32_t (&v)[16]
 }
 
 // Such a chunk through the epilogue.
+struct Output {
+  void* ptr;
+  int fp32, vec, vec8;
+};
+__device__ __forceinline__ Output output_of(const ProductArgs& p, const TileShape& s, int both_and_weight) {
+  return both_and_weight ? Output{p.out2, p.out2_fp32, s.vec2, s.vec8_2} : Output{p.epi.out, p.epi.out_fp32, s.vec, s.vec8};
+}
 template <bool kFinish>
-__device__ __forceinline__ void emit(const ProductArgs& p, const TileShape& shape, const Tile& c, int chunk, int f, float (&z)[16],
-                                     const Bias4& bias, const Residual4<4>& res) {
+__device__ __forceinline__ void emit(const ProductArgs& p, const TileShape& shape, const Output& out, const Tile& c, int chunk, int f,
+                                     float (&z)[16], const Bias4& bias, const Residual4<4>& res) {
   const int64_t row = c.out_row + chunk * 16 + ((threadIdx.x & 31) >> 3), last = c.out_row + c.valid;
   if (kFinish) {
     finish4<4>(p.epi, p.m, row, 4, last, f, z, bias, res, shape.vec);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (row + 4 * i < last) store4(p.epi.out, p.epi.out_fp32, p.epi.fp16, p.m, row + 4 * i, f, z + 4 * i, shape.vec);
+      if (row + 4 * i < last) store4(out.ptr, out.fp32, p.epi.fp16, p.m, row + 4 * i, f, z + 4 * i, out.vec);
   }
 }
 
@@ -181,7 +200,7 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
   Tile c{};
   bool ok = false;
   if (mine) {
-    c = locate<kKind>(worker, part, p, shape, t);
+    c = locate_tile<kKind>(worker, part, p, shape, t);
     ok = mbar_wait(smem_u32(&t->acc_full[0]), 0, ctx, 26);
     tc_fence_after();
   }
@@ -231,7 +250,7 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
         z[4 * i + 3] += from == part ? o[3] : q.w;
       }
     }
-    emit<kFinish>(p, shape, c, k, f, z, bias, res);
+    emit<kFinish>(p, shape, output_of(p, shape, 0), c, k, f, z, bias, res);
   }
 }
 
@@ -253,7 +272,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
 
   if (warp == 0) {
     if (lane < kMaxStages) {
-      mbar_init(smem_u32(&t->full[lane]), kKind == kWeightGrad ? 2 : 1);
+      mbar_init(smem_u32(&t->full[lane]), kKind >= kWeightGrad ? 2 : 1);
       mbar_init(smem_u32(&t->empty[lane]), 1);
       mbar_init(smem_u32(&t->raw[lane]), 1);
     }
@@ -265,6 +284,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
   } else if (warp == 1) {
     if (lane == 0) {
       prefetch_tmap(&maps.a);
+      if (kKind == kBothGrads) prefetch_tmap(&maps.a2);
       t->abort_flag = 0;
       t->max_len = 0;
       if (p.offsets == nullptr) {
@@ -323,6 +343,11 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     total_tiles = t->blocks[p.groups] * shape.f_tiles;
     half_rows = min(128, (t->max_len + 31) / 32 * 16);
   }
+  const int first_tiles = total_tiles;
+  if (kKind == kBothGrads) {
+    total_tiles += p.groups * shape.row_blocks * shape.f_tiles;
+    half_rows = max(half_rows, p.n <= 128 ? 64 : 128);
+  }
   const int stage_bytes = kABytes + max(half_rows, 16) * 128;
   const int stages = min(kMaxStages, int(kRingBytes) / stage_bytes);
   tc_fence_before();
@@ -341,16 +366,18 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     int stage = 0, round = 0;
     bool ok = true;
     for (int tile = worker; ok && tile < total_tiles; tile += workers) {
-      const Tile c = locate<kKind>(tile, part, p, shape, t);
+      const Tile c = locate<kKind>(tile, first_tiles, part, p, shape, t);
       const int steps = c.step1 - c.step0;
       if (elect_one()) {
         const int half = c.cols >> 1;
         const int f = c.f0 + int(rank) * 128, j = c.b_row + int(rank) * half;
         const uint32_t bytes = kABytes + half * 128;
-        const bool ragged = kKind == kWeightGrad && c.depth % kStep != 0;
-        int at = stage, turn = round;
+        const bool weight = kKind == kWeightGrad || (kKind == kBothGrads && c.weight);
+        const bool ragged = weight && c.depth % kStep != 0;
+        const CUtensorMap* map_a = kKind == kBothGrads && weight ? &maps.a2 : &maps.a;
+        int at = stage, lap = round;
         for (int kb = c.step0; kb < c.step1; ++kb) {
-          if (turn > 0 && !mbar_wait_lane(smem_u32(&t->empty[at]), (turn & 1) ^ 1, ctx, 21)) {
+          if (lap > 0 && !mbar_wait_lane(smem_u32(&t->empty[at]), (lap & 1) ^ 1, ctx, 21)) {
             ok = false;
             break;
           }
@@ -361,20 +388,18 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
             mbar_expect_tx(own_bar, bytes);
           } else if (rank == 0) {
             mbar_expect_tx(own_bar, 2 * bytes);
-            if (kKind == kWeightGrad) mbar_arrive(own_bar);
+            if (kKind >= kWeightGrad) mbar_arrive(own_bar);
           }
           const uint32_t a_dst = ring + at * stage_bytes, b_dst = a_dst + kABytes;
           const int k0 = kb * kStep;
           if (kKind == kForward) {
-            tma_load_3d_pair(a_dst, &maps.a, k0, f, c.group, bar);
-          } else if (kKind == kInputGrad) {
-            tma_load_3d_pair(a_dst, &maps.a, f, k0, c.group, bar);
-            tma_load_3d_pair(a_dst + 8192, &maps.a, f + 64, k0, c.group, bar);
+            tma_load_3d_pair(a_dst, map_a, k0, f, c.group, bar);
           } else {
-            tma_load_3d_pair(a_dst, &maps.a, f, c.c_begin + k0, 0, bar);
-            tma_load_3d_pair(a_dst + 8192, &maps.a, f + 64, c.c_begin + k0, 0, bar);
+            const int c1 = weight ? c.c_begin + k0 : k0, c2 = weight ? 0 : c.group;
+            tma_load_3d_pair(a_dst, map_a, f, c1, c2, bar);
+            tma_load_3d_pair(a_dst + 8192, map_a, f + 64, c1, c2, bar);
           }
-          if (kKind == kWeightGrad) {
+          if (weight) {
             tma_load_3d_pair(b_dst, &maps.b[2], j, c.c_begin + k0, 0, bar);
             if (half == 128) tma_load_3d_pair(b_dst + 8192, &maps.b[2], j + 64, c.c_begin + k0, 0, bar);
           } else {
@@ -386,7 +411,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
                 r += 16 << b;
               }
           }
-          if (++at == stages) { at = 0; ++turn; }
+          if (++at == stages) { at = 0; ++lap; }
         }
       }
       ok = __all_sync(0xffffffffu, ok);
@@ -401,36 +426,38 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     bool ok = true;
     const uint32_t fmt = p.epi.fp16 ? 0u : 1u;
     for (int tile = worker; rank == 0 && ok && tile < total_tiles; tile += workers, ++it) {
-      const Tile c = locate<kKind>(tile, part, p, shape, t);
+      const Tile c = locate<kKind>(tile, first_tiles, part, p, shape, t);
       const int steps = c.step1 - c.step0;
       if (elect_one()) {
         const uint32_t buf = it & 1, use = it >> 1;
         ok = mbar_wait_cluster_lane(smem_u32(&t->acc_empty[buf]), (use & 1) ^ 1, ctx, 22);
         tc_fence_after();
         const uint32_t d = tmem + buf * 256;
+        const bool weight = kKind == kWeightGrad || (kKind == kBothGrads && c.weight);
         const uint32_t idesc = make_idesc(fmt, fmt, 256, uint32_t(c.cols)) | (kKind != kForward ? 1u << 15 : 0u) |
-                               (kKind == kWeightGrad ? 1u << 16 : 0u);
-        int at = stage, turn = round;
-        uint32_t ready = steps > 0 ? mbar_peek_cluster(smem_u32(&t->full[at]), turn & 1) : 0;
+                               (weight ? 1u << 16 : 0u);
+        const int b_step = weight ? 128 : 2;
+        int at = stage, lap = round;
+        uint32_t ready = steps > 0 ? mbar_peek_cluster(smem_u32(&t->full[at]), lap & 1) : 0;
         for (int kb = c.step0; ok && kb < c.step1; ++kb) {
-          if (!ready && !mbar_wait_cluster_lane(smem_u32(&t->full[at]), turn & 1, ctx, 23)) {
+          if (!ready && !mbar_wait_cluster_lane(smem_u32(&t->full[at]), lap & 1, ctx, 23)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t a_addr = ring + at * stage_bytes;
           const uint64_t a_desc = kKind == kForward ? make_kmajor_sw128_desc(a_addr) : make_mnmajor_sw128_desc(a_addr);
-          const uint64_t b_desc = kKind == kWeightGrad ? make_mnmajor_sw128_desc(a_addr + kABytes)
+          const uint64_t b_desc = weight ? make_mnmajor_sw128_desc(a_addr + kABytes)
                                                        : make_kmajor_sw128_desc(a_addr + kABytes);
-          constexpr int kAStep = kKind == kForward ? 2 : 128, kBStep = kKind == kWeightGrad ? 128 : 2;
+          constexpr int kAStep = kKind == kForward ? 2 : 128;
           const int parts = min(4, (c.depth - kb * kStep + 15) / 16);
           const uint32_t empty_bar = smem_u32(&t->empty[at]);
-          if (++at == stages) { at = 0; ++turn; }
-          ready = kb + 1 < c.step1 ? mbar_peek_cluster(smem_u32(&t->full[at]), turn & 1) : 0;
+          if (++at == stages) { at = 0; ++lap; }
+          ready = kb + 1 < c.step1 ? mbar_peek_cluster(smem_u32(&t->full[at]), lap & 1) : 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             if (k < parts)
-              umma_h16_pair(d, a_desc + kAStep * k, b_desc + kBStep * k, idesc, kb > c.step0 || k > 0);
+              umma_h16_pair(d, a_desc + kAStep * k, b_desc + b_step * k, idesc, kb > c.step0 || k > 0);
           tc_commit_pair(empty_bar, pair_mask);
         }
         if (ok) tc_commit_pair(smem_u32(&t->acc_full[buf]), pair_mask);
@@ -444,10 +471,10 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     int stage = 0;
     uint32_t phases = 0;  // parity of raw[stage], one bit each
     bool ok = true;
-    for (int tile = worker; kKind == kWeightGrad && ok && tile < total_tiles; tile += workers) {
-      const Tile c = locate<kKind>(tile, part, p, shape, t);
+    for (int tile = worker; kKind >= kWeightGrad && ok && tile < total_tiles; tile += workers) {
+      const Tile c = locate<kKind>(tile, first_tiles, part, p, shape, t);
       const int last = c.depth / kStep;
-      if (c.depth % kStep != 0 && last >= c.step0 && last < c.step1) {
+      if ((kKind == kWeightGrad || c.weight) && c.depth % kStep != 0 && last >= c.step0 && last < c.step1) {
         const int at = (stage + last - c.step0) % stages;
         ok = mbar_wait(smem_u32(&t->raw[at]), (phases >> at) & 1, ctx, 24);
         if (!ok) break;
@@ -470,10 +497,11 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     }
   } else if (warp >= kFirstEpilogueWarp && shape.splits == 1) {
     // ---------------- epilogue: each warp on 32 features ----------------
-    float* turn = t->turn[warp - kFirstEpilogueWarp];
+    float* turn_block = t->turn[warp - kFirstEpilogueWarp];
     uint32_t it = 0;
     for (int tile = worker; tile < total_tiles; tile += workers, ++it) {
-      const Tile c = locate<kKind>(tile, part, p, shape, t);
+      const Tile c = locate<kKind>(tile, first_tiles, part, p, shape, t);
+      const Output out = output_of(p, shape, kKind == kBothGrads && c.weight);
       const uint32_t buf = it & 1, use = it >> 1;
       const int f = c.f0 + int(rank) * 128 + quarter * 32 + 4 * (lane & 7);
       Bias4 bias{};
@@ -488,12 +516,12 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
         if (lane == 0) mbar_arrive_cluster_relaxed(map_to_cta(smem_u32(&t->acc_empty[buf]), first_cta));
         released = true;
       };
-      if (shape.vec8 && summed) {
+      if (out.vec8 && summed) {
         // 16-bit outputs: two chunks at a time, read as fragments of 8x8 matrices (a lane has features 8m + lane / 4 of
         // two neighbouring output rows), finished in that layout, rounded two rows per instruction, transposed by stmatrix
         // into 1 KiB each ([row][32 features], the 16-byte pieces of a row XOR-swizzled) and stored 8 features per
         // thread.  The residual comes in the same way backwards, a pair of chunks ahead.
-        uint16_t* block = reinterpret_cast<uint16_t*>(turn);
+        uint16_t* block = reinterpret_cast<uint16_t*>(turn_block);
         const uint32_t st_addr = smem_u32(block) + uint32_t(lane & 7) * 64 + (uint32_t(lane >> 3) ^ ((lane >> 1) & 3u)) * 16;
         const int f8 = c.f0 + int(rank) * 128 + quarter * 32 + (lane & 3) * 8;
         // 16-byte piece i of this lane's four in a pair of chunks: its row and its place in `block`
@@ -510,13 +538,13 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
               res[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.epi.residual) +
                                                        (c.out_row + row_of(k, i)) * p.epi.residual_pitch + f8);
         };
-        auto store = [&](void* out, int k) {
+        auto store = [&](void* to, int k) {
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint4 q = *place_of(i);
             if (row_of(k, i) < c.valid && f8 < p.m)
-              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + (c.out_row + row_of(k, i)) * p.m + f8) = q;
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(to) + (c.out_row + row_of(k, i)) * p.m + f8) = q;
           }
           __syncwarp();
         };
@@ -563,7 +591,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
               for (int i = 0; i < 16; ++i) z[i] = __uint_as_float(v[u][i]);
               place(u, z);
             }
-            store(p.epi.out, k);
+            store(out.ptr, k);
             continue;
           }
           float z[2][16];
@@ -603,7 +631,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
           }
 #pragma unroll
           for (int u = 0; u < 2; ++u) place(u, z[u]);
-          store(p.epi.out, k);
+          store(out.ptr, k);
         }
       } else {
         // a chunk's share of the residual is requested one chunk ahead
@@ -622,8 +650,8 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
           tmem_ld_wait();
           if (k + 2 >= chunks) release();
           float z[16];
-          turn_chunk(turn, v, summed, z);
-          emit<kFinish>(p, shape, c, k, f, z, bias, res);
+          turn_chunk(turn_block, v, summed, z);
+          emit<kFinish>(p, shape, out, c, k, f, z, bias, res);
           res = next;
         }
       }
@@ -698,10 +726,21 @@ int make_map(CUtensorMap* map, const void* base, int64_t c0, int64_t c1, int64_t
 bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 using KernelFn = void (*)(const Maps, const ProductArgs, const TileShape);
-template <int kKind>
-KernelFn kernel_of(bool finish) {
-  if (kKind == kForward && finish) return product_kernel<kForward, true>;
-  return product_kernel<kKind, false>;
+KernelFn kernel_of(ProductKind kind, bool finish) {
+  switch (kind) {
+    case kForward: return finish ? product_kernel<kForward, true> : product_kernel<kForward, false>;
+    case kInputGrad: return product_kernel<kInputGrad, false>;
+    case kWeightGrad: return product_kernel<kWeightGrad, false>;
+    default: return product_kernel<kBothGrads, false>;
+  }
+}
+
+// Tiles that there can be.
+int64_t most_tiles(ProductKind kind, const ProductArgs& p) {
+  const int64_t f_tiles = ceil_div(p.m, kTileFeatures);
+  if (kind == kWeightGrad) return p.groups * ceil_div(p.n, kTileRows) * f_tiles;
+  // a segment's last block may be short: at most one more per segment than the rows fill
+  return (p.offsets ? int64_t(p.rows) / kTileRows + std::min(p.groups, p.rows) : ceil_div(p.rows, kTileRows)) * f_tiles;
 }
 
 }  // namespace
@@ -717,51 +756,77 @@ int product_status(int* status_out, int clear, cudaStream_t stream) {
 int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaStream_t stream) {
   const int sms = device_sm_count(device);
   MB200_REQUIRE(sms > 1, kCudaError, "product: cannot read the SM count of device %d", device);
-  const bool weight = kind == kWeightGrad;
+  const bool weight = kind == kWeightGrad, both = kind == kBothGrads;
   TileShape s{};
   s.f_tiles = int(ceil_div(args.m, kTileFeatures));
-  s.row_blocks = weight ? int(ceil_div(args.n, kTileRows)) : 0;
-  // a segment's last block may be short: at most one more per segment than the rows fill
-  const int64_t blocks = weight ? int64_t(args.groups) * s.row_blocks
-                         : args.offsets ? int64_t(args.rows) / kTileRows + std::min(args.groups, args.rows)
-                                        : ceil_div(args.rows, kTileRows);
-  const int64_t tiles = blocks * s.f_tiles;
+  s.row_blocks = weight || both ? int(ceil_div(args.n, kTileRows)) : 0;
+  const int64_t tiles = most_tiles(both ? kInputGrad : kind, args) + (both ? most_tiles(kWeightGrad, args) : 0);
   MB200_REQUIRE(tiles < (int64_t(1) << 30), kUnsupportedShape, "product: %lld tiles do not fit 32-bit tile numbers",
                 (long long)tiles);
   const Epilogue& e = args.epi;
-  s.vec = epilogue_vec(e, args.m);
   const bool finish = e.bias || e.act || e.residual || e.slope;
+  s.vec = epilogue_vec(e, args.m);
   s.vec8 = !e.out_fp32 && args.m % 8 == 0 && aligned_to(e.out, 16) && aligned_to(e.slope, 16) &&
            (!e.residual || (aligned_to(e.residual, 16) && e.residual_pitch % 8 == 0));
+  s.vec2 = args.m % 4 == 0 && aligned_to(args.out2, args.out2_fp32 ? 16 : 8);
+  s.vec8_2 = !args.out2_fp32 && args.m % 8 == 0 && aligned_to(args.out2, 16);
 
-  Maps maps;
+  Maps maps{};
   int rc;
   const int fp16 = e.fp16;
   if (kind == kForward) rc = make_map(&maps.a, args.a, args.k, args.m, args.groups, args.a_pitch, args.a_group, 128, fp16);
-  else if (kind == kInputGrad) rc = make_map(&maps.a, args.a, args.m, args.k, args.groups, args.a_pitch, args.a_group, 64, fp16);
+  else if (!weight) rc = make_map(&maps.a, args.a, args.m, args.k, args.groups, args.a_pitch, args.a_group, 64, fp16);
   else rc = make_map(&maps.a, args.a, args.m, args.rows, 1, args.a_pitch, 0, 64, fp16);
+  if (!rc && both) rc = make_map(&maps.a2, args.a2, args.m, args.rows, 1, args.a2_pitch, 0, 64, fp16);
   if (rc) return rc;
-  for (int i = 0; i < kBoxes; ++i)
+  // boxes of 64 columns of b; the weight gradient takes those of 64 rows
+  for (int i = weight ? 2 : 0; i < (weight ? 3 : kBoxes); ++i)
     if ((rc = make_map(&maps.b[i], args.b, weight ? args.n : args.k, args.rows, 1, args.b_pitch, 0, 16u << i, fp16))) return rc;
 
-  const int variant = kind == kForward ? (finish ? 1 : 0) : kind == kInputGrad ? 2 : 3;
-  const KernelFn kernel = kind == kForward     ? kernel_of<kForward>(finish)
-                          : kind == kInputGrad ? kernel_of<kInputGrad>(false)
-                                               : kernel_of<kWeightGrad>(false);
-  static std::atomic<bool> configured[kMaxDevices][4];
+  const int variant = kind == kForward ? (finish ? 1 : 0) : kind + 1;
+  const KernelFn kernel = kernel_of(kind, finish);
+  static std::atomic<bool> configured[kMaxDevices][5];
   if (device < 0 || device >= kMaxDevices || !configured[device][variant].load(std::memory_order_acquire)) {
     MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)));
     MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     if (device >= 0 && device < kMaxDevices) configured[device][variant].store(true, std::memory_order_release);
   }
   // beyond half of the pairs nothing is split: the launch need not ask
-  s.splits = tiles * 2 > sms / 2
+  s.splits = both || tiles * 2 > sms / 2
                  ? 1
                  : split_count(reinterpret_cast<const void*>(kernel), tiles, ceil_div(weight ? args.rows / args.groups : args.k, kStep), device);
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = cluster_config(int(std::min(tiles, int64_t(sms / 2))), s.splits, stream, attr);
   MB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps, args, s));
   return kOk;
+}
+
+int launch_gradients(const ProductArgs& args, void* dx, void* dw, int dw_fp32, const void* w, int64_t w_pitch, int64_t w_group,
+                     const void* x, int64_t x_pitch, int device, cudaStream_t stream) {
+  ProductArgs p = args;
+  p.a = w;
+  p.a_pitch = w_pitch;
+  p.a_group = w_group;
+  p.epi.out = dx;
+  const int64_t pairs = device_sm_count(device) / 2;
+  // Dense: one launch for both, unless one has so few tiles that its sums are better split (4096 x 7168 -> 2048: 208 us
+  // with one, 231 with two).  Ragged segments: two, since reading all experts' weights and writing all their gradients at once
+  // takes longer than one after the other (32 experts of 1024 rows: 3.49 against 3.37 ms).
+  if (dx && dw && !p.offsets && most_tiles(kInputGrad, p) * 2 > pairs && most_tiles(kWeightGrad, p) * 2 > pairs) {
+    p.a2 = x;
+    p.a2_pitch = x_pitch;
+    p.out2 = dw;
+    p.out2_fp32 = dw_fp32;
+    return launch_product(kBothGrads, p, device, stream);
+  }
+  int rc;
+  if (dx && (rc = launch_product(kInputGrad, p, device, stream))) return rc;
+  if (!dw) return kOk;
+  p.a = x;
+  p.a_pitch = x_pitch;
+  p.epi.out = dw;
+  p.epi.out_fp32 = dw_fp32;
+  return launch_product(kWeightGrad, p, device, stream);
 }
 
 }  // namespace mb200
