@@ -137,12 +137,12 @@ __device__ __forceinline__ void take_apart(const Vec<T, kVec> (&v)[kPer], Pair (
   }
 }
 
+// `to`: this thread's first vector of the output row
 template <typename T, int kVec, int kPer>
-__device__ __forceinline__ void store_row(T* row, int64_t hidden, const Pair (&p)[kVec * kPer / 2]) {
+__device__ __forceinline__ void store_row(T* to, uint32_t mask, const Pair (&p)[kVec * kPer / 2]) {
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    const int64_t at = int64_t(threadIdx.x + k * blockDim.x) * kVec;
-    if (at < hidden) {
+    if (mask >> k & 1) {
       Vec<T, kVec> o;
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
@@ -155,7 +155,7 @@ __device__ __forceinline__ void store_row(T* row, int64_t hidden, const Pair (&p
           o.v[i] = from_float<T>(f[e & 1]);
         }
       }
-      *reinterpret_cast<Vec<T, kVec>*>(row + at) = o;
+      *reinterpret_cast<Vec<T, kVec>*>(to + k * int(blockDim.x) * kVec) = o;
     }
   }
 }
@@ -210,38 +210,57 @@ __device__ __forceinline__ void row_sums(float (&v)[kCount], float (*part)[32][2
 // that nothing but its own wait stands between copy and use), or where single elements are copied the next row in registers.
 // Columns past the row's end and rows past the last read as zero.
 constexpr int kStages = 3;
-template <typename T, int kVec, int kPer>
+template <typename T, int kVec, int kPer, int kTensors>
 struct RowStream {
   static constexpr bool kShared = kVec > 1;
-  const T* base;
-  int64_t pitch, rows, hidden;
-  uint32_t slot;           // this thread's first vector of stage 0
-  uint32_t stage_bytes;
-  Vec<T, kVec> ahead[kShared ? 1 : kPer];
+  static constexpr int kAhead = kShared ? kStages : 1;
+  const T* next[kTensors];     // this thread's first vector of the next row to ask for
+  int64_t row_step[kTensors];  // elements to the one after it
+  int rows_left;               // rows that this thread's group has still to ask for
+  uint32_t mask;               // which of its vectors lie inside the row
+  uint32_t slot, vec_bytes;    // its first vector of stage 0, bytes from one to the next
+  Vec<T, kVec> ahead[kShared ? 1 : kTensors][kPer];
 
-  __device__ __forceinline__ RowStream(const void* p, int64_t pitch_, int64_t rows_, int64_t hidden_, uint32_t smem, int which, int streams)
-      : base(reinterpret_cast<const T*>(p)), pitch(pitch_), rows(rows_), hidden(hidden_) {
-    const uint32_t threads = blockDim.x * blockDim.y, thread = threadIdx.y * blockDim.x + threadIdx.x;
-    stage_bytes = threads * kPer * 16 * streams;
-    slot = smem + which * threads * kPer * 16 + thread * 16;
-  }
-  __device__ __forceinline__ void request(int64_t row, int stage) {
-    const T* p = base + row * pitch;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int64_t at = int64_t(threadIdx.x + k * blockDim.x) * kVec;
-      const bool inside = row < rows && at < hidden;
-      if constexpr (kShared) {
-        const uint32_t to = slot + stage * stage_bytes + k * blockDim.x * blockDim.y * 16;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(inside ? p + at : base), "r"(inside ? 16 : 0)
-                     : "memory");
-      } else {
-        ahead[k] = Vec<T, kVec>{};
-        if (inside) ahead[k] = load_once<T, kVec>(p + at);
-      }
+  __device__ __forceinline__ RowStream(const void* p0, int64_t pitch0, const void* p1, int64_t pitch1, int64_t first_row, int64_t step,
+                                       int64_t rows, uint32_t mask_, uint32_t smem)
+      : mask(mask_) {
+    rows_left = first_row < rows ? int((rows - first_row + step - 1) / step) : 0;
+    const int64_t row = rows_left > 0 ? first_row : 0;
+    next[0] = reinterpret_cast<const T*>(p0) + row * pitch0 + int(threadIdx.x) * kVec;
+    row_step[0] = step * pitch0;
+    if constexpr (kTensors > 1) {
+      next[1] = reinterpret_cast<const T*>(p1) + row * pitch1 + int(threadIdx.x) * kVec;
+      row_step[1] = step * pitch1;
     }
+    vec_bytes = blockDim.x * blockDim.y * 16;
+    slot = smem + (threadIdx.y * blockDim.x + threadIdx.x) * 16;
   }
-  __device__ __forceinline__ void take(int stage, Pair (&out)[kVec * kPer / 2]) {
+  __device__ __forceinline__ void request(int stage) {
+    const uint32_t here = rows_left > 0 ? mask : 0u;
+#pragma unroll
+    for (int n = 0; n < kTensors; ++n)
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const bool inside = here >> k & 1;
+        const T* from = next[n] + k * int(blockDim.x) * kVec;
+        if constexpr (kShared) {
+          const uint32_t to = slot + ((stage * kTensors + n) * kPer + k) * vec_bytes;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(inside ? from : next[n]), "r"(inside ? 16 : 0)
+                       : "memory");
+        } else {
+          ahead[n][k] = Vec<T, kVec>{};
+          if (inside) ahead[n][k] = load_once<T, kVec>(from);
+        }
+      }
+    if constexpr (kShared) asm volatile("cp.async.commit_group;" ::: "memory");
+    --rows_left;
+#pragma unroll
+    for (int n = 0; n < kTensors; ++n) next[n] += rows_left > 0 ? row_step[n] : 0;
+  }
+  __device__ __forceinline__ void wait() {
+    if constexpr (kShared) asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+  }
+  __device__ __forceinline__ void take(int n, int stage, Pair (&out)[kVec * kPer / 2]) {
     if constexpr (kShared) {
       Vec<T, kVec> v[kPer];
 #pragma unroll
@@ -249,17 +268,15 @@ struct RowStream {
         uint32_t* w = reinterpret_cast<uint32_t*>(&v[k]);
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "r"(slot + stage * stage_bytes + k * blockDim.x * blockDim.y * 16)
+                     : "r"(slot + ((stage * kTensors + n) * kPer + k) * vec_bytes)
                      : "memory");
       }
       take_apart<T, kVec, kPer>(v, out);
     } else {
-      take_apart<T, kVec, kPer>(ahead, out);
+      take_apart<T, kVec, kPer>(ahead[n], out);
     }
   }
 };
-__device__ __forceinline__ void stream_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void stream_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
 
 // Which of a thread's vectors lie inside the row, and how many elements its warp and the warp with the number of its lane
 // have; the same for every row.
@@ -352,24 +369,21 @@ __global__ void __launch_bounds__(kMaxThreads, kBlocks) norm_kernel(const NormAr
   const int64_t step = int64_t(gridDim.x) * blockDim.y;
   const float inv = 1.f / float(p.hidden);
   int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  using Stream = RowStream<T, kVec, kPer>;
-  constexpr int kAhead = Stream::kShared ? kStages : 1;
-  Stream x(p.x, p.x_pitch, p.rows, p.hidden, smem_u32(rows_smem), 0, 1);
-  for (int i = 0; i < kAhead; ++i) {
-    x.request(r + i * step, i);
-    stream_commit();
-  }
+  using Stream = RowStream<T, kVec, kPer, 1>;
+  constexpr int kAhead = Stream::kAhead;
   const RowShare<kVec, kPer> share(p.hidden);
+  Stream x(p.x, p.x_pitch, nullptr, 0, r, step, p.rows, share.mask, smem_u32(rows_smem));
+  T* to = reinterpret_cast<T*>(p.out) + r * p.hidden + int(threadIdx.x) * kVec;
+  for (int i = 0; i < kAhead; ++i) x.request(i);
   Pair w[kPairs], b[kPairs];
   load_params<T, kVec, kPer>(p.weight, p.params_fp32, p.hidden, 1.f, w);
   load_params<T, kVec, kPer>(p.bias, p.params_fp32, p.hidden, 0.f, b);
   // all rows of a block take the same number of turns: its threads meet at the barriers
   for (int64_t first = int64_t(blockIdx.x) * blockDim.y; first < p.rows; first += step, r += step) {
     Pair v[kPairs];
-    if (Stream::kShared) stream_wait();
-    x.take(stage, v);
-    x.request(r + kAhead * step, stage);
-    stream_commit();
+    x.wait();
+    x.take(0, stage, v);
+    x.request(stage);
     stage = stage + 1 == kAhead ? 0 : stage + 1;
     float mean, squares;
     row_moments<kVec, kPer>(v, share, inv, part, turn, mean, squares);
@@ -378,7 +392,8 @@ __global__ void __launch_bounds__(kMaxThreads, kBlocks) norm_kernel(const NormAr
       const Pair m2 = pair_of(-mean, -mean), r2 = pair_of(rstd, rstd);
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) v[i] = fma2(mul2(add2(v[i], m2), r2), w[i], b[i]);
-      store_row<T, kVec, kPer>(reinterpret_cast<T*>(p.out) + r * p.hidden, p.hidden, v);
+      store_row<T, kVec, kPer>(to, share.mask, v);
+      to += step * p.hidden;
       if (threadIdx.x == 0) {
         p.mean[r] = mean;
         p.rstd[r] = rstd;
@@ -398,26 +413,24 @@ __global__ void __launch_bounds__(kMaxThreads) norm_grad_kernel(const NormArgs p
   const int64_t step = int64_t(gridDim.x) * blockDim.y;
   const float inv = 1.f / float(p.hidden);
   int64_t r = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  using Stream = RowStream<T, kVec, kPer>;
-  constexpr int kAhead = Stream::kShared ? kStages : 1;
-  Stream x(p.x, p.x_pitch, p.rows, p.hidden, smem_u32(rows_smem), 0, 2);
-  Stream dy(p.dy, p.dy_pitch, p.rows, p.hidden, smem_u32(rows_smem), 1, 2);
-  for (int i = 0; i < kAhead; ++i) {
-    x.request(r + i * step, i);
-    dy.request(r + i * step, i);
-    stream_commit();
-  }
+  using Stream = RowStream<T, kVec, kPer, 2>;
+  constexpr int kAhead = Stream::kAhead;
+  uint32_t mask = 0;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k)
+    if (int64_t(threadIdx.x + k * blockDim.x) * kVec < p.hidden) mask |= 1u << k;
+  Stream stream(p.x, p.x_pitch, p.dy, p.dy_pitch, r, step, p.rows, mask, smem_u32(rows_smem));
+  T* to = reinterpret_cast<T*>(p.out) + r * p.hidden + int(threadIdx.x) * kVec;
+  for (int i = 0; i < kAhead; ++i) stream.request(i);
   float mean = r < p.rows ? __ldg(p.mean + r) : 0.f, rstd = r < p.rows ? __ldg(p.rstd + r) : 0.f;
   Pair w[kPairs], dw[kPairs] = {}, db[kPairs] = {};
   load_params<T, kVec, kPer>(p.weight, p.params_fp32, p.hidden, 1.f, w);
   for (int64_t first = int64_t(blockIdx.x) * blockDim.y; first < p.rows; first += step, r += step) {
     Pair h[kPairs], g[kPairs];
-    if (Stream::kShared) stream_wait();
-    x.take(stage, h);
-    dy.take(stage, g);
-    x.request(r + kAhead * step, stage);
-    dy.request(r + kAhead * step, stage);
-    stream_commit();
+    stream.wait();
+    stream.take(0, stage, h);
+    stream.take(1, stage, g);
+    stream.request(stage);
     stage = stage + 1 == kAhead ? 0 : stage + 1;
     const Pair m2 = pair_of(-mean, -mean), r2 = pair_of(rstd, rstd);
     const bool here = r < p.rows;
@@ -441,7 +454,8 @@ __global__ void __launch_bounds__(kMaxThreads) norm_grad_kernel(const NormArgs p
         const Pair a2 = pair_of(-s[0] * inv, -s[0] * inv), b2 = pair_of(-s[1] * inv, -s[1] * inv);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) g[i] = mul2(r2, fma2(h[i], b2, add2(g[i], a2)));
-        store_row<T, kVec, kPer>(reinterpret_cast<T*>(p.out) + r * p.hidden, p.hidden, g);
+        store_row<T, kVec, kPer>(to, mask, g);
+        to += step * p.hidden;
       }
     }
   }
@@ -576,11 +590,12 @@ constexpr Shape kForwardVec[] = {{2, 64, 1024}, {4, 256, 512}, {4, 512, 512}};
 constexpr Shape kForwardVecFew[] = {{1, 1024, 1024}, {4, 512, 512}};
 constexpr Shape kForwardOne[] = {{4, 256, 1024}, {16, 1024, 1024}};
 constexpr Shape kForwardOneFew[] = {{4, 1024, 1024}, {16, 1024, 1024}};
-constexpr Shape kBackwardVec[] = {{1, 512, 1024}, {2, 512, 512}};
-constexpr Shape kBackwardVecFew[] = {{1, 1024, 1024}, {2, 512, 512}};
+// 16-bit rows of 16384 elements keep part of their column sums in local memory: 179 us for 4096 of them, where the kernel for
+// rows of any length takes 571
+constexpr Shape kBackwardVec[] = {{2, 512, 512}, {4, 512, 512}};
+constexpr Shape kBackwardVecFew[] = {{1, 1024, 1024}, {2, 512, 512}, {4, 512, 512}};
 constexpr Shape kBackwardOne[] = {{4, 512, 1024}, {16, 512, 512}};
 constexpr Shape kBackwardOneFew[] = {{4, 1024, 1024}, {16, 512, 512}};
-constexpr Shape kBackwardVec32 = {4, 512, 512};  // fp32 only: 16-bit rows of that length spill their sums
 
 template <size_t kCount>
 bool pick(const Shape (&shapes)[kCount], int64_t vecs, Shape& out) {
@@ -601,14 +616,10 @@ Plan make_plan(bool backward, int elem_bytes, bool aligned, int64_t rows, int64_
   const int64_t vecs = (hidden + l.vec - 1) / l.vec;
   Shape s;
   const bool few = rows <= sms;
-  bool found = backward ? (aligned ? (few ? pick(kBackwardVecFew, vecs, s) : pick(kBackwardVec, vecs, s))
+  const bool found = backward ? (aligned ? (few ? pick(kBackwardVecFew, vecs, s) : pick(kBackwardVec, vecs, s))
                                          : (few ? pick(kBackwardOneFew, vecs, s) : pick(kBackwardOne, vecs, s)))
                               : (aligned ? (few ? pick(kForwardVecFew, vecs, s) : pick(kForwardVec, vecs, s))
                                          : (few ? pick(kForwardOneFew, vecs, s) : pick(kForwardOne, vecs, s)));
-  if (!found && backward && aligned && elem_bytes == 4 && vecs <= kBackwardVec32.per * kBackwardVec32.most) {
-    s = kBackwardVec32;
-    found = true;
-  }
   if (!found) {
     l.vec = 0;
     l.block = dim3(kLongThreads);
@@ -644,9 +655,7 @@ KernelFn backward_kernel(const Plan& l) {
   if (l.vec == 0) return norm_grad_long_kernel<T>;
   if (l.vec == 1) return l.per == 4 ? norm_grad_kernel<T, 1, 4, 1024> : norm_grad_kernel<T, 1, 16, 512>;
   if (l.per == 1) return norm_grad_kernel<T, kV, 1, 1024>;
-  if constexpr (sizeof(T) == 4)
-    if (l.per == 4) return norm_grad_kernel<T, kV, 4, 512>;
-  return norm_grad_kernel<T, kV, 2, 512>;
+  return l.per == 2 ? norm_grad_kernel<T, kV, 2, 512> : norm_grad_kernel<T, kV, 4, 512>;
 }
 
 int launch(bool backward, int precision, const NormArgs& a, const Plan& l, int device, cudaStream_t stream) {
