@@ -117,6 +117,15 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_gated_front_end_needs_a_gpu():
+    from moe_bench_b200 import gating
+    from moe_bench_b200 import problem as P
+
+    cfg = P.MoEBenchConfig(hidden_size=64, intermediate_size=64, num_experts=4, topk=2, world_size=1, device="cpu")
+    with pytest.raises(capi.MB200Error, match="CUDA"):
+        gating.make_gated_problem(cfg, 4)
+
+
 # ---- the oracle itself ----
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
 def test_oracle_linear_gradients_are_autograds_and_differences(act):
