@@ -205,7 +205,7 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
     tc_fence_after();
   }
   __syncwarp();
-  cluster_sync();  // every pair's products have read their stages
+  cluster_sync_relaxed();  // every pair's products have read their stages
   const bool summed = c.step1 > c.step0;
   const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
   const int chunks = (c.valid + 15) >> 4;
@@ -217,10 +217,14 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
       uint32_t v[16];
       tmem_ld16(lanes + k * 16, v);
       tmem_ld_wait();
-      const uint32_t to = map_to_cta(ring + block_of(k, part), uint32_t(k % splits) * 2 + (cta & 1)) + lane * 4;
+      float z[16];
+      turn_chunk(t->turn[warp - kFirstEpilogueWarp], v, summed, z);
+      const uint32_t to = map_to_cta(ring + block_of(k, part), uint32_t(k % splits) * 2 + (cta & 1)) + (lane >> 3) * 128 + (lane & 7) * 16;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + i * 128), "r"(summed ? v[i] : 0u) : "memory");
+      for (int i = 0; i < 4; ++i)
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + i * 512), "f"(z[4 * i]), "f"(z[4 * i + 1]),
+                     "f"(z[4 * i + 2]), "f"(z[4 * i + 3])
+                     : "memory");
     }
   }
   __syncwarp();
@@ -668,7 +672,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     // a wait was abandoned: copies and products still in flight get time to land
     for (int i = 0; i < 64; ++i) __nanosleep(1000);
   }
-  cluster_sync();  // the other CTA arrives on this one's barriers no more
+  cluster_sync_relaxed();  // the other CTA arrives on this one's barriers no more
   tc_fence_after();
   if (warp == 3) tmem_dealloc_pair(tmem, kTmemCols);
 }
