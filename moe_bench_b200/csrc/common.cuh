@@ -415,6 +415,20 @@ __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The wait for one or two chunks of 16 registers.  The arrays are named as in/out operands so that no use of them, not even
+// one that touches registers alone, moves above the wait.
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait16x2(uint32_t (&v)[2][16]) {
+  tmem_ld_wait16(v[0]);
+  tmem_ld_wait16(v[1]);
+}
+
 // 32 lanes x 32 consecutive fp32 columns -> 32 registers per thread.  The load is
 // asynchronous: the registers hold the data only after tmem_ld_wait32 on the same array.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {

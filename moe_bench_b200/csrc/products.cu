@@ -216,7 +216,7 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
       if (k % splits == part) continue;
       uint32_t v[16];
       tmem_ld16(lanes + k * 16, v);
-      tmem_ld_wait();
+      tmem_ld_wait16(v);
       float z[16];
       turn_chunk(t->turn[warp - kFirstEpilogueWarp], v, summed, z);
       const uint32_t to = map_to_cta(ring + block_of(k, part), uint32_t(k % splits) * 2 + (cta & 1)) + (lane >> 3) * 128 + (lane & 7) * 16;
@@ -238,7 +238,7 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
     if (kFinish) res = load_residual4<4>(p.epi, p.m, c.out_row + k * 16 + (lane >> 3), 4, c.out_row + c.valid, f, shape.vec);
     uint32_t v[16];
     tmem_ld16(lanes + k * 16, v);
-    tmem_ld_wait();
+    tmem_ld_wait16(v);
     float own[16], z[16] = {};
     turn_chunk(t->turn[warp - kFirstEpilogueWarp], v, summed, own);
     for (int from = 0; from < splits; ++from) {
@@ -422,6 +422,11 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
       round += (stage + steps) / stages;
       stage = (stage + steps) % stages;
     }
+    // the products' last arrivals come from the pair's first CTA: this one is not gone before they are here
+    for (int i = 0; ok && i < stages; ++i) {
+      if (round > 0) ok = mbar_wait(smem_u32(&t->empty[stage]), (round & 1) ^ 1, ctx, 21);
+      if (++stage == stages) { stage = 0; ++round; }
+    }
   } else if (warp == 1) {
     // ---------------- products (the pair's first CTA) ----------------
     // One thread again; it asks for the next step while this one's products are issued.
@@ -470,6 +475,11 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
       round += (stage + steps) / stages;
       stage = (stage + steps) % stages;
     }
+    // nor before the other CTA's last arrivals on its accumulators (none where parts are joined)
+    if (rank == 0 && ok && shape.splits == 1 && elect_one())
+      for (uint32_t b = 0; b < 2 && b < it; ++b)
+        mbar_wait_cluster_lane(smem_u32(&t->acc_empty[b]), ((it - 1 - b) >> 1) & 1, ctx, 22);
+    __syncwarp();
   } else if (warp == 2) {
     // ---------------- weight gradient: rows past the segment's end become zeros ----------------
     int stage = 0;
@@ -585,7 +595,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
               tmem_ld_frag16(lanes + (k + 2 * u) * 16, v[u]);
               tmem_ld_frag16(lanes + (k + 2 * u) * 16 + (16u << 16), v[u] + 8);
             }
-          tmem_ld_wait();
+          tmem_ld_wait16x2(v);
           if (k + 4 >= chunks) release();
           if (!kFinish) {
 #pragma unroll
@@ -651,7 +661,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
           Residual4<4> next{};
           if (kFinish && k + 2 < chunks)
             next = load_residual4<4>(p.epi, p.m, c.out_row + (k + 2) * 16 + (lane >> 3), 4, last, f, shape.vec);
-          tmem_ld_wait();
+          tmem_ld_wait16(v);
           if (k + 2 >= chunks) release();
           float z[16];
           turn_chunk(turn_block, v, summed, z);

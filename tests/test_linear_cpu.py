@@ -179,3 +179,36 @@ def test_prototypes_match_the_header(lib):
         args = re.search(r"\b%s\s*\(([^)]*)\)" % name, text).group(1).split(",")
         got = ["*" if "*" in a else a.split()[0] for a in args]
         assert got == [kinds[c] for c in capi.SIGNATURES[name][1]], name
+
+
+# ---- what no run can be made to show: the sources are held to it ----
+def _source(name):
+    import os
+    import re
+
+    return re.sub(r"//[^\n]*", "", open(os.path.join(mb_build.CSRC, name)).read())
+
+
+def test_products_poll_through_the_bounded_waits_only():
+    text = _source("products.cu") + _source("few_rows.cu") + _source("linear.cuh")
+    assert "try_wait" not in text and "test_wait" not in text and "while (true)" not in text
+
+
+def test_no_cta_leaves_before_its_last_remote_arrivals():
+    """Arrivals from the pair's other CTA (the products' commits on `empty`, the epilogue's on `acc_empty`) are waited for after the
+    loops, ahead of the cluster barrier that ends the kernel."""
+    text = _source("products.cu")
+    end = text.rindex("cluster_sync_relaxed();")
+    loads, products = text.index("int stage = 0, round = 0;"), text.rindex("int stage = 0, round = 0;")
+    masks = text.index("} else if (warp == 2) {")
+    after_loads = text[text.rindex("stage = (stage + steps) % stages;", loads, products) : products]
+    assert "mbar_wait(smem_u32(&t->empty[stage])" in after_loads
+    after_products = text[text.rindex("stage = (stage + steps) % stages;", products, masks) : masks]
+    assert "mbar_wait_cluster_lane(smem_u32(&t->acc_empty[b])" in after_products
+    assert masks < end
+
+
+def test_tensor_memory_is_used_only_behind_waits_that_name_the_registers():
+    text = _source("products.cu")
+    assert "tmem_ld_wait();" not in text
+    assert text.count("tmem_ld16(") == text.count("tmem_ld_wait16(v)") == 3 and text.count("tmem_ld_wait16x2(v)") == 1
