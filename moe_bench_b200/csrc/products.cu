@@ -15,9 +15,13 @@
 // operands, so that NaN and infinities there reach nothing.
 //
 // 384 threads: warp 0 loads, warp 1 of the pair's first CTA issues the products, warp 2 clears those tails,
-// warps 4-11 drain the accumulators (two sets, so that the next tile's products run meanwhile): 32 features x 16
-// output rows at a time go through a 2 KiB block of shared memory that turns them round, still in fp32, and leave
-// through the epilogue as 64 contiguous bytes per output row.  Every wait is bounded.
+// warps 4-11 drain the accumulators (two sets, so that the next tile's products run meanwhile).  A lane holds one
+// feature of many output rows, memory wants many features of one row: where outputs are of 16 bits and start on 16 bytes, 32
+// features x 32 output rows at a time are read as fragments, finished, rounded and transposed by stmatrix; else 32 x 16
+// go through a 2 KiB block of shared memory still in fp32.  Every wait is bounded.
+//
+// Few tiles leave pairs idle, so up to eight pairs form a cluster and share a tile, each with a part of its sums; the parts
+// meet in shared memory and are added in the pairs' order (join_parts).
 
 #include <algorithm>
 #include <atomic>
@@ -347,6 +351,8 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     total_tiles = t->blocks[p.groups] * shape.f_tiles;
     half_rows = min(128, (t->max_len + 31) / 32 * 16);
   }
+  // a cluster that joins parts has one tile at most; only offsets that do not ascend could ask for more
+  if (shape.splits > 1) total_tiles = min(total_tiles, workers);
   const int first_tiles = total_tiles;
   if (kKind == kBothGrads) {
     total_tiles += p.groups * shape.row_blocks * shape.f_tiles;

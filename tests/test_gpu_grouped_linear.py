@@ -103,6 +103,20 @@ def test_offsets_past_the_rows_are_cut():
     assert torch.equal(capi.grouped_linear(x, w, low), capi.grouped_linear(x, w, _offsets([10, 30, 0])))
 
 
+def test_segments_that_overlap_end_all_the_same():
+    """Offsets that do not ascend name more rows than there are; whatever comes out, every wait completes, and calls after it
+    are right."""
+    g = _gen(31)
+    x, w = _normal(g, 4096, 512), _normal(g, 8, 64, 512, scale=0.05)
+    dy = _normal(g, 4096, 64)
+    bad = torch.tensor([0, 4096, 0, 4096, 0, 4096, 0, 4096, 0], device=DEV, dtype=torch.int32)
+    y = capi.grouped_linear(x, w, bad)
+    dx, dw = capi.grouped_linear_backward(dy, x, w, bad)
+    assert capi.linear_status() == 0 and y.shape == dy.shape and dx.shape == x.shape and dw.shape == w.shape
+    sizes = [512] * 8
+    _good(capi.grouped_linear(x, w, _offsets(sizes)), F.grouped_linear(x, w, sizes), "y")
+
+
 def test_half_of_fused_weights_and_pitches():
     g = _gen(5)
     w1, x = _normal(g, 6, 2 * 40, 96, scale=0.1), _normal(g, 90, 200)[:, 8:104]
