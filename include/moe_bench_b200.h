@@ -346,6 +346,8 @@ int mb200_read_status(const void* workspace, int32_t* status_out, void* stream);
  *    the operands of products (x, w, and dy unless it has to be copied, see there) start on a
  *    16-byte boundary and have pitches that are multiples of 8 elements, and k is a multiple
  *    of 8; n, rows and segment lengths are any; outputs are dense (pitch = columns);
+ *  - what a call writes lies apart from everything else it is given (checked), but for the
+ *    in-place forms named below;
  *  - calls that share no output and no workspace may overlap; a workspace (16-byte aligned, no
  *    initial contents needed) is free again when the call's work on the stream is done;
  *  - results do not depend on what else runs: every sum has a fixed order;
@@ -361,7 +363,7 @@ int mb200_read_status(const void* workspace, int32_t* status_out, void* stream);
  * bias_fp32, else the precision's type) or NULL; residual [rows, n] or NULL; y [rows, n], fp32
  * if out_fp32.  slope: NULL, or [rows, n] in the precision's type that receives act'(z), the
  * one thing of the forward that the backward call below needs besides x and w.  y may be the
- * residual's buffer (same type and pitch n). */
+ * residual itself (same type and pitch n). */
 int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, const void* w, int64_t w_pitch,
                  int n, int k, const void* bias, int bias_fp32, int activation, const void* residual,
                  int64_t residual_pitch, void* y, int out_fp32, void* slope, int device, void* stream);
@@ -408,7 +410,8 @@ int mb200_linear_status(int32_t* status_out, int clear, void* stream);
  * fp32 (variance about the mean, divided by hidden), y = (x - mean) * rstd * weight + bias.
  * x [rows, hidden], y [rows, hidden] dense; weight, bias [hidden] or NULL.  precision also takes
  * MB200_PRECISION_FP32 here, the type of x, y, weight and bias alike; params_fp32: weight and
- * bias are fp32 whatever x is.  Any hidden from 1 up, any pitch >= hidden. */
+ * bias are fp32 whatever x is.  Any hidden from 1 up, any pitch >= hidden.  y may be x itself
+ * (pitch hidden). */
 #define MB200_PRECISION_FP32 3
 int mb200_layer_norm(int precision, const void* x, int64_t x_pitch, int64_t rows, int64_t hidden, const void* weight,
                      const void* bias, int params_fp32, float eps, void* y, float* mean, float* rstd, int device,

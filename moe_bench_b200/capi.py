@@ -740,7 +740,8 @@ def _norm_operands(x, weight, bias, name: str):
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     """Layer norm of the rows of ``x [rows, hidden]`` (bf16, fp16 or fp32; rows may be any distance apart): returns
-    ``(y, mean, rstd)``, the last two in fp32 for ``layer_norm_backward``.  weight and bias have x's type or fp32."""
+    ``(y, mean, rstd)``, the last two in fp32 for ``layer_norm_backward``.  weight and bias have x's type or fp32.
+    ``out`` may be a contiguous x itself."""
     dev = x.get_device()
     if _elsewhere(dev):
         with torch.cuda.device(dev):

@@ -721,6 +721,14 @@ int mb200_layer_norm(int precision, const void* x, int64_t x_pitch, int64_t rows
                 (long long)hidden);
   if (rows == 0) return kOk;
   MB200_REQUIRE(x && y && mean && rstd, kInvalidArgument, "layer_norm: null pointer");
+  const int size = precision == MB200_PRECISION_FP32 ? 4 : 2, param_size = params_fp32 ? 4 : size;
+  // y = x is fine: a row is written by the threads that have read it, and no other row reads it
+  const bool in_place = y == x && (x_pitch == hidden || rows == 1);
+  if ((rc = check_apart("layer_norm",
+                        {span_of("y", y, rows, hidden, hidden, size), span_of("mean", mean, 1, rows, rows, 4), span_of("rstd", rstd, 1, rows, rows, 4)},
+                        {span_of("x", in_place ? nullptr : x, rows, x_pitch, hidden, size),
+                         span_of("weight", weight, 1, hidden, hidden, param_size), span_of("bias", bias, 1, hidden, hidden, param_size)})))
+    return rc;
   NormArgs a{};
   a.x = x;
   a.x_pitch = x_pitch;
@@ -734,7 +742,6 @@ int mb200_layer_norm(int precision, const void* x, int64_t x_pitch, int64_t rows
   a.mean = mean;
   a.rstd = rstd;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int size = precision == MB200_PRECISION_FP32 ? 4 : 2;
   const Plan l = make_plan(false, size, rows_aligned(a, size), rows, hidden, device);
   return launch(false, precision, a, l, device, s);
 }
@@ -787,6 +794,14 @@ int mb200_layer_norm_backward(int precision, const void* dy, int64_t dy_pitch, c
                   (long long)workspace_bytes, (long long)need);
     a.sums = reinterpret_cast<float*>(workspace);
   }
+  if ((rc = check_apart("layer_norm_backward",
+                        {span_of("dx", dx, rows, hidden, hidden, size), span_of("dweight", dweight, 1, hidden, hidden, 4),
+                         span_of("dbias", dbias, 1, hidden, hidden, 4),
+                         span_of("workspace", a.sums, int64_t(l.parts) * 2, hidden, hidden, 4)},
+                        {span_of("dy", dy, rows, dy_pitch, hidden, size), span_of("x", x, rows, x_pitch, hidden, size),
+                         span_of("mean", mean, 1, rows, rows, 4), span_of("rstd", rstd, 1, rows, rows, 4),
+                         span_of("weight", weight, 1, hidden, hidden, params_fp32 ? 4 : size)})))
+    return rc;
   if ((rc = launch(true, precision, a, l, device, s))) return rc;
   if (a.sums) return launch_column_sums(a.sums, l.parts, 2 * hidden, dweight, hidden, dbias, s);
   return kOk;

@@ -168,19 +168,31 @@ int check_groups(int experts, const int32_t* offsets, int64_t expert_pitch, int6
   return kOk;
 }
 
-// dy itself, or the copy of it (times slope) in the workspace that the products read; db on the way.
-int prepare_output_grad(const char* what, const void*& dy, int dy_fp32, int64_t& dy_pitch, const void* slope,
-                        int64_t rows, int n, int fp16, bool products, float* db, void* workspace,
-                        int64_t workspace_bytes, int device, cudaStream_t s) {
-  int rc;
-  const bool copy = products && (slope || dy_fp32 || dy_pitch % 8 || !aligned16(dy));
-  if (!copy && !db) return kOk;
+// Whether the products read a copy of dy (times slope), in the workspace.
+bool copies_output_grad(const void* dy, int dy_fp32, int64_t dy_pitch, const void* slope) {
+  return slope || dy_fp32 || dy_pitch % 8 || !aligned16(dy);
+}
+
+// `need`: bytes of the workspace that the call uses
+int check_grad_workspace(const char* what, bool copy, bool sums, int64_t rows, int n, const void* workspace, int64_t workspace_bytes,
+                         int device, int64_t& need) {
+  need = 0;
+  if (!copy && !sums) return kOk;
   const GradLayout l = grad_layout(rows, n, device);
-  const int64_t need = (copy ? l.dz_bytes : 0) + (db ? l.sum_bytes : 0);
+  need = (copy ? l.dz_bytes : 0) + (sums ? l.sum_bytes : 0);
   MB200_REQUIRE(need == 0 || (workspace && aligned16(workspace)), kInvalidArgument,
                 "%s: needs a 16-byte aligned workspace", what);
   MB200_REQUIRE(workspace_bytes >= need, kWorkspaceTooSmall, "%s: workspace %lld < %lld bytes", what,
                 (long long)workspace_bytes, (long long)need);
+  return kOk;
+}
+
+// dy itself, or the copy of it (times slope) in the workspace that the products read; db on the way.
+int prepare_output_grad(const void*& dy, int dy_fp32, int64_t& dy_pitch, const void* slope, int64_t rows, int n, int fp16, bool copy,
+                        float* db, void* workspace, int device, cudaStream_t s) {
+  int rc;
+  if (!copy && !db) return kOk;
+  const GradLayout l = grad_layout(rows, n, device);
   char* ws = reinterpret_cast<char*>(workspace);
   OutputGrad g{};
   g.dy = dy;
@@ -240,6 +252,12 @@ int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, co
   if (rows == 0) return kOk;
   if ((rc = check_operand(x, x_pitch, k, what, "x")) || (rc = check_operand(w, w_pitch, k, what, "w"))) return rc;
   MB200_REQUIRE(y != nullptr, kInvalidArgument, "linear: y is null");
+  const bool in_place = residual == y && !out_fp32 && (residual_pitch == n || rows == 1);
+  if ((rc = check_apart(what, {span_of("y", y, rows, n, n, out_fp32 ? 4 : 2), span_of("slope", slope, rows, n, n, 2)},
+                        {span_of("x", x, rows, x_pitch, k, 2), span_of("w", w, n, w_pitch, k, 2),
+                         span_of("bias", bias, 1, n, n, bias_fp32 ? 4 : 2),
+                         span_of("residual", in_place ? nullptr : residual, rows, residual_pitch, n, 2)})))
+    return rc;
   ProductArgs p{};
   p.a = w;
   p.a_pitch = w_pitch;
@@ -286,9 +304,16 @@ int mb200_linear_backward(int precision, const void* dy, int dy_fp32, int64_t dy
   MB200_REQUIRE(dy != nullptr, kInvalidArgument, "linear_backward: dy is null");
   if (dx && (rc = check_operand(w, w_pitch, k, what, "w"))) return rc;
   if (dw && (rc = check_operand(x, x_pitch, k, what, "x"))) return rc;
-  if ((rc = prepare_output_grad(what, dy, dy_fp32, dy_pitch, slope, rows, n, fp16, dx || dw, db, workspace,
-                                workspace_bytes, device, s)))
+  const bool copy = (dx || dw) && copies_output_grad(dy, dy_fp32, dy_pitch, slope);
+  int64_t need;
+  if ((rc = check_grad_workspace(what, copy, db, rows, n, workspace, workspace_bytes, device, need)) ||
+      (rc = check_apart(what,
+                        {span_of("dx", dx, rows, k, k, 2), span_of("dw", dw, n, k, k, dw_fp32 ? 4 : 2), span_of("db", db, 1, n, n, 4),
+                         span_of("workspace", workspace, 1, need, need, 1)},
+                        {span_of("dy", dy, rows, dy_pitch, n, dy_fp32 ? 4 : 2), span_of("slope", slope, rows, n, n, 2),
+                         span_of("x", dw ? x : nullptr, rows, x_pitch, k, 2), span_of("w", dx ? w : nullptr, n, w_pitch, k, 2)})))
     return rc;
+  if ((rc = prepare_output_grad(dy, dy_fp32, dy_pitch, slope, rows, n, fp16, copy, db, workspace, device, s))) return rc;
   ProductArgs p{};
   p.b = dy;
   p.b_pitch = dy_pitch;
@@ -312,6 +337,10 @@ int mb200_grouped_linear(int precision, const void* x, int64_t x_pitch, int64_t 
   if (rows == 0) return kOk;
   if ((rc = check_operand(x, x_pitch, k, what, "x")) || (rc = check_operand(w, w_pitch, k, what, "w"))) return rc;
   MB200_REQUIRE(y != nullptr, kInvalidArgument, "grouped_linear: y is null");
+  if ((rc = check_apart(what, {span_of("y", y, rows, n, n, 2)},
+                        {span_of("x", x, rows, x_pitch, k, 2), span_of("w", w, experts, w_expert_pitch, (n - 1) * w_pitch + k, 2),
+                         span_of("offsets", offsets, 1, 0, experts + 1, 4)})))
+    return rc;
   ProductArgs p{};
   p.a = w;
   p.a_pitch = w_pitch;
@@ -350,9 +379,17 @@ int mb200_grouped_linear_backward(int precision, const void* dy, int64_t dy_pitc
   MB200_REQUIRE(dy != nullptr, kInvalidArgument, "grouped_linear_backward: dy is null");
   if (dx && (rc = check_operand(w, w_pitch, k, what, "w"))) return rc;
   if (dw && (rc = check_operand(x, x_pitch, k, what, "x"))) return rc;
-  if ((rc = prepare_output_grad(what, dy, 0, dy_pitch, nullptr, rows, n, fp16, dx || dw, nullptr, workspace,
-                                workspace_bytes, device, s)))
+  const bool copy = (dx || dw) && copies_output_grad(dy, 0, dy_pitch, nullptr);
+  int64_t need;
+  if ((rc = check_grad_workspace(what, copy, false, rows, n, workspace, workspace_bytes, device, need)) ||
+      (rc = check_apart(what,
+                        {span_of("dx", dx, rows, k, k, 2), span_of("dw", dw, int64_t(experts) * n, k, k, dw_fp32 ? 4 : 2),
+                         span_of("workspace", workspace, 1, need, need, 1)},
+                        {span_of("dy", dy, rows, dy_pitch, n, 2), span_of("x", dw ? x : nullptr, rows, x_pitch, k, 2),
+                         span_of("w", dx ? w : nullptr, experts, w_expert_pitch, (n - 1) * w_pitch + k, 2),
+                         span_of("offsets", offsets, 1, 0, experts + 1, 4)})))
     return rc;
+  if ((rc = prepare_output_grad(dy, 0, dy_pitch, nullptr, rows, n, fp16, copy, nullptr, workspace, device, s))) return rc;
   ProductArgs p{};
   p.b = dy;
   p.b_pitch = dy_pitch;

@@ -2,6 +2,8 @@
 // and both gradients, dense (one group) or over ragged row segments, and the epilogue they share.
 #pragma once
 
+#include <initializer_list>
+
 #include "layer.cuh"
 
 namespace mb200 {
@@ -197,6 +199,31 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int m, int64_t row, i
 inline int epilogue_vec(const Epilogue& e, int m) {
   auto at = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
   return m % 4 == 0 && at(e.out, e.out_fp32 ? 16 : 8) && at(e.slope, 8) && (!e.residual || (at(e.residual, 8) && e.residual_pitch % 4 == 0));
+}
+
+// The memory that a call writes must be apart from all other memory it is given: a kernel reads its inputs while it writes.
+struct Span {
+  const char* name;
+  uintptr_t begin, end;  // empty where there is no tensor
+};
+inline Span span_of(const char* name, const void* p, int64_t rows, int64_t pitch, int64_t cols, int64_t bytes) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  return {name, at, p == nullptr || rows <= 0 ? at : at + uintptr_t(((rows - 1) * pitch + cols) * bytes)};
+}
+inline int check_apart(const char* what, std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  auto check = [what](const Span& a, const Span& b) -> int {
+    MB200_REQUIRE(a.begin >= b.end || b.begin >= a.end || a.begin == a.end || b.begin == b.end, kInvalidArgument,
+                  "%s: %s and %s share memory", what, a.name, b.name);
+    return kOk;
+  };
+  int rc;
+  for (const Span* w = written.begin(); w != written.end(); ++w) {
+    for (const Span& r : read)
+      if ((rc = check(*w, r))) return rc;
+    for (const Span* v = w + 1; v != written.end(); ++v)
+      if ((rc = check(*w, *v))) return rc;
+  }
+  return kOk;
 }
 
 // layer_norm.cu

@@ -88,6 +88,14 @@ def test_a_spoilt_row_spoils_no_other():
     assert torch.isnan(y[7]).all() and torch.isnan(y[11]).all()
 
 
+@pytest.mark.parametrize("rows,hidden", [(5, 7), (900, 64), (1500, 520), (40, 7168), (700, 7168), (600, 1031), (6, 40000)])
+def test_in_place(rows, hidden):
+    g = _gen(rows)
+    x, w, b = (torch.randn(*s, device=DEV, generator=g).bfloat16() for s in ((rows, hidden), (hidden,), (hidden,)))
+    expect = capi.layer_norm(x, w, b)
+    assert all(torch.equal(a, c) for a, c in zip(capi.layer_norm(x, w, b, out=x), expect))
+
+
 def test_single_gradients_and_no_rows():
     g = _gen(2)
     x, dy = torch.randn(30, 200, device=DEV, generator=g).bfloat16(), torch.randn(30, 200, device=DEV, generator=g).bfloat16()

@@ -100,6 +100,59 @@ def test_norm_refuses(lib):
     assert back(0, P, 64, P, 64, 2, 64, None, P, None, 0, P, P, P, P, 1 << 20, 0, None) != 0 and b"null" in lib.mb200_last_error()
 
 
+# x 4 x 64, w 5 x 64, y 4 x 5 and so on, each on a megabyte of its own unless the case says otherwise
+MB = 1 << 20
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(y=MB), b"y and x share"), (dict(y=MB + 4 * 64 * 2 - 2), b"y and x share"), (dict(y=2 * MB + 5 * 64 * 2 - 8), b"y and w share"),
+    (dict(y=3 * MB, bias=3 * MB + 16), b"y and bias share"), (dict(y=MB - 4 * 5 * 2 + 2), b"y and x share"),
+    (dict(res=3 * MB, rp=8), b"y and residual share"), (dict(res=3 * MB + 2, rp=5), b"y and residual share"),
+    (dict(res=3 * MB, rp=5, o32=1), b"y and residual share"), (dict(slope=3 * MB), b"y and slope share"),
+    (dict(slope=MB), b"slope and x share"),
+])
+def test_linear_refuses_to_write_what_it_reads(lib, change, words):
+    assert _linear(lib, **{**dict(x=MB, w=2 * MB, y=3 * MB), **change}) != 0
+    assert words in lib.mb200_last_error()
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(dx=MB), b"dx and dy share"), (dict(dx=2 * MB), b"dx and x share"), (dict(dx=3 * MB), b"dx and w share"),
+    (dict(dw=2 * MB), b"dw and x share"), (dict(dw=4 * MB), b"dx and dw share"), (dict(db=6 * MB + 8), b"db and workspace share"),
+    (dict(db=8 * MB), b"db and slope share"), (dict(ws=8 * MB), b"workspace and slope share"),
+])
+def test_linear_backward_refuses_to_write_what_it_reads(lib, change, words):
+    apart = dict(dy=MB, x=2 * MB, w=3 * MB, dx=4 * MB, dw=5 * MB, ws=6 * MB, db=7 * MB, slope=8 * MB)
+    assert _linear_backward(lib, **{**apart, **change}) != 0
+    assert words in lib.mb200_last_error()
+
+
+def test_grouped_refuses_to_write_what_it_reads(lib):
+    apart = dict(x=MB, w=2 * MB, off=3 * MB, y=4 * MB)
+    for change, words in ((dict(y=MB), b"y and x share"), (dict(y=2 * MB + (2 * 5 + 4) * 64 * 2), b"y and w share"),
+                          (dict(off=4 * MB + 32), b"y and offsets share")):
+        assert _grouped(lib, **{**apart, **change}) != 0 and words in lib.mb200_last_error()
+    back = lib.mb200_grouped_linear_backward
+    for dx, dw, words in ((MB, 8 * MB, b"dx and dy share"), (7 * MB, 2 * MB + 64, b"dw and x share"), (3 * MB, 8 * MB, b"dx and w share"),
+                          (8 * MB + 2 * 8 * 64 * 2, 8 * MB, b"dx and dw share")):
+        assert back(0, MB, 8, 2 * MB, 64, 4, 3 * MB, 64, 64 * 8, 4 * MB, 3, 8, 64, dx, dw, 0, None, 0, 0, None) != 0
+        assert words in lib.mb200_last_error()
+
+
+def test_norm_refuses_to_write_what_it_reads(lib):
+    def call(x=MB, xp=64, w=2 * MB, y=3 * MB, m=4 * MB, r=5 * MB):
+        return lib.mb200_layer_norm(0, x, xp, 2, 64, w, None, 1, 1e-5, y, m, r, 0, None)
+
+    for kw, words in ((dict(y=MB, xp=72), b"y and x share"), (dict(y=MB + 2), b"y and x share"), (dict(y=2 * MB + 128), b"y and weight share"),
+                      (dict(m=5 * MB + 4), b"mean and rstd share"), (dict(r=MB), b"rstd and x share")):
+        assert call(**kw) != 0 and words in lib.mb200_last_error()
+    back = lib.mb200_layer_norm_backward
+    for dx, dwt, words in ((MB, 8 * MB, b"dx and dy share"), (2 * MB, 8 * MB, b"dx and x share"), (7 * MB, 3 * MB, b"dweight and mean share"),
+                           (7 * MB, 9 * MB, b"dweight and workspace share")):
+        assert back(0, MB, 64, 2 * MB, 64, 2, 64, 3 * MB, 4 * MB, None, 0, dx, dwt, None, 9 * MB, MB, 0, None) != 0
+        assert words in lib.mb200_last_error()
+
+
 def test_workspace_queries_refuse_bad_sizes(lib):
     assert lib.mb200_linear_backward_workspace_bytes(4, 0, 1, 0) == -1
     assert lib.mb200_grouped_linear_backward_workspace_bytes(-1, 8) == -1
