@@ -301,7 +301,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
         t->blocks[0] = 0;
         t->blocks[1] = (p.rows + kTileRows - 1) / kTileRows;
       }
-    } else if (lane <= kBoxes) {
+    } else if (kKind == kWeightGrad ? lane == 3 : lane <= kBoxes) {
       prefetch_tmap(&maps.b[lane - 1]);
     }
   } else if (warp == 3) {

@@ -167,6 +167,46 @@ def test_gated_front_end_feeds_the_layer():
     assert torch.equal(again.topk_ids, prob.topk_ids) and torch.equal(again.hidden_states, prob.hidden_states)
 
 
+def test_threads_with_streams_of_their_own():
+    """Four host threads, each with its stream, tensors and sizes: nothing but the device is shared, and every result is the
+    one that the calls give alone."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    def operands(i):
+        g = torch.Generator(device=DEV)
+        g.manual_seed(i)
+        rows, k, n = 300 + 137 * i, 1024, 256 + 8 * i
+        t = [(torch.randn(*s, device=DEV, generator=g) * 0.1).bfloat16() for s in ((rows, k), (n, k), (rows, n), (3, n, k), (k,))]
+        return t + [torch.tensor([0, 100, 100, rows], device=DEV, dtype=torch.int32)]
+
+    def calls(t):
+        x, w, dy, experts, gain, off = t
+        y, slope = capi.linear(x, w, activation="silu", want_slope=True)
+        out = [y, slope, capi.linear(x[:5], w), *capi.linear_backward(dy, x, w, slope=slope), capi.grouped_linear(x, experts, off)]
+        out += capi.grouped_linear_backward(dy, x, experts, off)
+        h, mean, rstd = capi.layer_norm(x, gain)
+        return out + [h, mean, rstd, *capi.layer_norm_backward(x, x, mean, rstd, gain)]
+
+    sets = [operands(i) for i in range(4)]
+    alone = [calls(t) for t in sets]
+    torch.cuda.synchronize()
+
+    def work(t):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            results = [calls(t) for _ in range(20)]
+        stream.synchronize()
+        return results
+
+    with ThreadPoolExecutor(4) as pool:
+        together = list(pool.map(work, sets))
+    for expect, many in zip(alone, together):
+        for got in many:
+            assert all(torch.equal(a, b) for a, b in zip(got, expect))
+    assert capi.linear_status() == 0
+
+
+
 FIRST_CALLS = """
 import torch
 from moe_bench_b200 import capi
