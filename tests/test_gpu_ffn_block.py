@@ -11,6 +11,7 @@ import torch
 from moe_bench_b200 import capi, gating
 from moe_bench_b200 import problem as P
 from moe_bench_b200.plugin import get_implementation
+from oracle import ffn_oracle as F
 from oracle import moe_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -240,3 +241,52 @@ def test_first_calls_of_a_process_may_be_captured():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     res = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=180)
     assert res.returncode == 0 and "fine" in res.stdout, res.stderr[-2000:]
+
+
+def test_tensors_of_more_elements_than_32_bits_count():
+    """Rows repeat, so that every element of the large results has a known value; gradients come from the last rows alone."""
+    rows, n, k, period = 128 * 2064, 16400, 8, 128
+    assert rows * n > 1 << 32
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+
+    def normal(*shape):
+        return torch.randn(*shape, device=DEV, generator=g).bfloat16()
+
+    def repeats(t, expect):
+        return all(torch.equal(t[i : i + 16 * period].view(-1, period, t.shape[1]), expect.expand(16, *expect.shape))
+                   for i in range(0, rows, 16 * period))
+
+    w, few, bias, tail = normal(n, k), normal(period, k), normal(n), normal(100, n)
+    x = few.repeat(rows // period, 1)
+    y = capi.linear(x, w, bias)
+    assert not F.inside(y[:period], *F.linear(few, w, bias, "none", None, y.dtype)[:2]) and repeats(y, y[:period].clone())
+    dy = y.zero_()
+    dy[-100:] = tail
+    slope = torch.ones_like(dy)
+    expect = F.linear_backward(tail, x[-100:], w, slope[:100], w.dtype)
+    for s in (None, slope):  # with a slope the products read a copy of dy
+        dx, dw, db = capi.linear_backward(dy, x, w, slope=s)
+        assert not dx[:-100].any()
+        for got, ref in zip((dx[-100:], dw, db), expect):
+            assert not F.inside(got, *ref)
+    del slope
+    experts = torch.stack([w, w.flip(0), -w])
+    off = torch.tensor([0, rows - 50, rows - 50, rows], device=DEV, dtype=torch.int32)
+    out = capi.grouped_linear(x, experts, off, out=dy)
+    front = capi.linear(few, w)
+    assert torch.equal(out[-50:], -front[-50:])
+    out[-50:] = front[-50:]
+    assert repeats(out, front)
+    h = out[:, : n - 16]  # rows apart
+    few_h = h[:period]
+    h, (one, mean, rstd) = capi.layer_norm(h), capi.layer_norm(few_h)
+    assert repeats(h[0], one) and torch.equal(h[1].view(-1, period), mean.expand(rows // period, period))
+    dh = torch.zeros_like(h[0])
+    dh[-100:] = tail[:, : n - 16]
+    got = capi.layer_norm_backward(dh, out[:, : n - 16], h[1], h[2])
+    assert not got[0][:-100].any()
+    alone = F.layer_norm_backward(dh[-100:], few_h[-100:], mean[-100:], rstd[-100:], None)
+    for a, r in zip((got[0][-100:], *got[1:]), alone):
+        assert not F.inside(a, *r)
+    assert capi.linear_status() == 0
