@@ -187,7 +187,7 @@ __device__ __forceinline__ void load_params(const void* p, int fp32, int64_t hid
 }
 
 // Sums of kCount values over a row's threads, the same in all of them.  The calls of a block take the two halves of
-// `part` in turn, so that one barrier is enough.
+// `part` in turn, so that one barrier is enough: of the row's own threads, where a block takes several rows side by side.
 template <int kCount>
 __device__ __forceinline__ void row_sums(float (&v)[kCount], float (*part)[32][2], int& turn) {
 #pragma unroll
@@ -199,7 +199,7 @@ __device__ __forceinline__ void row_sums(float (&v)[kCount], float (*part)[32][2
   if (lane == 0)
 #pragma unroll
     for (int c = 0; c < kCount; ++c) part[turn][threadIdx.x >> 5][c] = v[c];
-  __syncthreads();
+  asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
 #pragma unroll
   for (int c = 0; c < kCount; ++c) v[c] = lane < warps ? part[turn][lane][c] : 0.f;
   turn ^= 1;
@@ -405,13 +405,27 @@ __global__ void __launch_bounds__(kMaxThreads, kBlocks) norm_kernel(const NormAr
   }
 }
 
+constexpr int kMostRows = 8;  // rows that a block takes side by side at most
+
+template <int kCount>
+__device__ __forceinline__ void store_floats(float* to, const float (&f)[kCount]) {
+  if constexpr (kCount % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < kCount; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) to[i] = f[i];
+  }
+}
+
 // Every thread keeps the sums of its columns over the rows it sees, and leaves them in `sums` at the end.  Columns past
 // the row's end have dy = 0, so they add nothing to any sum.
 template <typename T, int kVec, int kPer, int kMaxThreads>
 __global__ void __launch_bounds__(kMaxThreads) norm_grad_kernel(const NormArgs p) {
   constexpr int kPairs = kVec * kPer / 2;
   extern __shared__ __align__(16) uint8_t rows_smem[];
-  __shared__ float part[2][32][2];
+  __shared__ float parts[kMostRows][2][32][2];
+  float (*part)[32][2] = parts[threadIdx.y];
   int turn = 0, stage = 0;
   const int64_t step = int64_t(gridDim.x) * blockDim.y;
   const float inv = 1.f / float(p.hidden);
@@ -463,21 +477,38 @@ __global__ void __launch_bounds__(kMaxThreads) norm_grad_kernel(const NormArgs p
     }
   }
   if (p.sums == nullptr) return;
-  float* sums = p.sums + (int64_t(blockIdx.x) * blockDim.y + threadIdx.y) * 2 * p.hidden;
+  // a block's sums of dy*h, then of dy; the rows that it takes side by side are added first, in order
+  float* sums = p.sums + int64_t(blockIdx.x) * 2 * p.hidden;
+  float* to_smem = reinterpret_cast<float*>(rows_smem) + threadIdx.y * 2 * kPer * kVec * blockDim.x;
+  if (blockDim.y > 1) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+  }
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    const int64_t at = int64_t(threadIdx.x + k * blockDim.x) * kVec;
-    if (at < p.hidden) {
+    const int at = int(threadIdx.x + k * blockDim.x) * kVec;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float f[kVec];
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
-        const int e = k * kVec + i;
-        float f[2];
-        unpack_f32x2(dw[e / 2], f[0], f[1]);
-        sums[at + i] = f[e & 1];
-        unpack_f32x2(db[e / 2], f[0], f[1]);
-        sums[p.hidden + at + i] = f[e & 1];
+        float both[2];
+        unpack_f32x2(which ? db[(k * kVec + i) / 2] : dw[(k * kVec + i) / 2], both[0], both[1]);
+        f[i] = both[(k * kVec + i) & 1];
       }
+      if (blockDim.y > 1) store_floats(to_smem + which * kPer * kVec * blockDim.x + at, f);
+      else if (at < p.hidden) store_floats(sums + which * p.hidden + at, f);
     }
+  }
+  if (blockDim.y == 1) return;
+  __syncthreads();
+  const int padded = kPer * kVec * blockDim.x;
+  for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < 2 * padded; c += blockDim.x * blockDim.y) {
+    const int which = c >= padded, at = c - which * padded;
+    if (at >= p.hidden) continue;
+    float t = 0.f;
+    for (int y = 0; y < int(blockDim.y); ++y) t += reinterpret_cast<const float*>(rows_smem)[y * 2 * padded + c];
+    sums[which * p.hidden + at] = t;
   }
 }
 
@@ -551,26 +582,38 @@ __global__ void __launch_bounds__(kLongThreads) norm_grad_long_kernel(const Norm
   }
 }
 
-// Parts added in a fixed order, 32 columns x 32 lanes per block: lane k takes parts k, k + 32, ..., then the lanes in order.
+// Parts added in a fixed order, 32 kWidth columns x 32 lanes per block: lane k takes parts k, k + 32, ..., then the lanes' sums by
+// a tree.  Bound by the second launch and by the latency of its loads: 148 parts of 14336 columns (8.5 MB, which lie in L2)
+// 5 us after the kernel before, 6 with one column per thread.
 constexpr int kSumLanes = 32;
+template <int kWidth>
 __global__ void __launch_bounds__(32 * kSumLanes) column_sums_kernel(const float* parts, int count, int64_t columns, float* out,
                                                                      int64_t first, float* rest) {
-  __shared__ float lanes[kSumLanes][33];
+  __shared__ Vec<float, kWidth> lanes[kSumLanes][33];
   const int c = threadIdx.x & 31, lane = threadIdx.x >> 5;
-  const int64_t i = int64_t(blockIdx.x) * 32 + c;
-  float s = 0.f;
+  const int64_t i = (int64_t(blockIdx.x) * 32 + c) * kWidth;
+  Vec<float, kWidth> s{};
   if (i < columns)
 #pragma unroll 4
-    for (int k = lane; k < count; k += kSumLanes) s += parts[k * columns + i];
+    for (int k = lane; k < count; k += kSumLanes) {
+      const Vec<float, kWidth> v = *reinterpret_cast<const Vec<float, kWidth>*>(parts + k * columns + i);
+#pragma unroll
+      for (int e = 0; e < kWidth; ++e) s.v[e] += v.v[e];
+    }
   lanes[lane][c] = s;
   __syncthreads();
-  s = warp_sum(lanes[c][lane]);  // this warp's column, one lane's sum per thread
-  const int64_t at = int64_t(blockIdx.x) * 32 + lane;
-  if (c != 0 || at >= columns) return;
+  s = lanes[c][lane];  // this warp's columns, one lane's sums per thread
+#pragma unroll
+  for (int e = 0; e < kWidth; ++e) s.v[e] = warp_sum(s.v[e]);
+  const int64_t at = (int64_t(blockIdx.x) * 32 + lane) * kWidth + c;
+  if (c >= kWidth || at >= columns) return;
+  float mine = s.v[0];
+#pragma unroll
+  for (int e = 1; e < kWidth; ++e) mine = c == e ? s.v[e] : mine;
   if (at < first) {
-    if (out) out[at] = s;
+    if (out) out[at] = mine;
   } else if (rest) {
-    rest[at - first] = s;
+    rest[at - first] = mine;
   }
 }
 
@@ -591,7 +634,9 @@ struct Shape {
 };
 constexpr Shape kForwardVec[] = {{2, 64, 1024}, {4, 256, 512}, {4, 512, 512}};
 constexpr Shape kForwardVecFew[] = {{1, 1024, 1024}, {4, 512, 512}};
-constexpr Shape kForwardOne[] = {{4, 256, 1024}, {16, 1024, 1024}};
+// single elements, 1777 rows of 1031: 7.7 us with four per thread, 14.2 with sixteen; past 2048 it is the other way (20000 rows
+// of 2049: 83 against 112)
+constexpr Shape kForwardOne[] = {{4, 512, 1024}, {16, 1024, 1024}};
 constexpr Shape kForwardOneFew[] = {{4, 1024, 1024}, {16, 1024, 1024}};
 // 16-bit rows of 16384 elements keep part of their column sums in local memory: 172 us for 4096 of them, where the kernel for
 // rows of any length takes 571
@@ -633,13 +678,16 @@ Plan make_plan(bool backward, int elem_bytes, bool aligned, int64_t rows, int64_
   l.per = s.per;
   l.most = s.most;
   const int tpr = int((vecs + l.per - 1) / l.per + 31) / 32 * 32;
-  l.block = dim3(tpr, tpr == 32 ? 8 : 1);
+  // Rows of one warp go eight to a block; backward, where a block leaves sums for a second kernel to add, also rows of up to four
+  // warps, side by side (10000 rows of 1536: 31 -> 21 us, 3000 of 1024 13.7 -> 9.5; of eight warps 19.6 -> 21.1, so not there)
+  const bool side_by_side = tpr == 32 || (backward && !few && tpr <= 128);
+  l.block = dim3(tpr, side_by_side ? std::min(kMostRows, s.most / tpr) : 1);
   const int threads = tpr * int(l.block.y);
   int resident = s.threads_per_sm / threads;
   resident = resident < 1 ? 1 : resident;
   const int64_t wanted = (rows + l.block.y - 1) / l.block.y;
   l.blocks = int(wanted < int64_t(sms) * resident ? wanted : int64_t(sms) * resident);
-  l.parts = l.blocks * int(l.block.y);
+  l.parts = l.blocks;
   return l;
 }
 
@@ -666,13 +714,14 @@ int launch(bool backward, int precision, const NormArgs& a, const Plan& l, int d
   const KernelFn kernel = type == 0   ? (backward ? backward_kernel<float>(l) : forward_kernel<float>(l))
                           : type == 1 ? (backward ? backward_kernel<__half>(l) : forward_kernel<__half>(l))
                                       : (backward ? backward_kernel<__nv_bfloat16>(l) : forward_kernel<__nv_bfloat16>(l));
-  const size_t smem = l.vec > 1 ? size_t(kStages) * l.block.x * l.block.y * l.per * 16 * (backward ? 2 : 1) : 0;
+  size_t smem = l.vec > 1 ? size_t(kStages) * l.block.x * l.block.y * l.per * 16 * (backward ? 2 : 1) : 0;
+  if (backward && a.sums && l.block.y > 1) smem = std::max(smem, size_t(l.block.x) * l.block.y * l.per * l.vec * 2 * 4);
   if (smem > 40 * 1024) {  // with the static share past the 48 KiB that need no asking
     // the most any plan takes, once per device and kernel; a second thread that sets it again does no harm
     static std::atomic<bool> configured[kMaxDevices][2][3][5];
     std::atomic<bool>* done = device >= 0 && device < kMaxDevices ? &configured[device][backward][type][l.per] : nullptr;
     if (!done || !done->load(std::memory_order_acquire)) {
-      MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024));
+      MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
       if (done) done->store(true, std::memory_order_release);
     }
   }
@@ -700,8 +749,13 @@ int check_norm(int precision, int64_t rows, int64_t hidden, const char* what) {
 
 }  // namespace
 
+// Four columns per thread as soon as half of the SMs get a block.
+constexpr int kWide = 64;
 int launch_column_sums(const float* parts, int count, int64_t columns, float* out, int64_t first, float* rest, cudaStream_t stream) {
-  column_sums_kernel<<<unsigned((columns + 31) / 32), 32 * kSumLanes, 0, stream>>>(parts, count, columns, out, first, rest);
+  if (columns % 4 == 0 && columns >= 128 * kWide && (reinterpret_cast<uintptr_t>(parts) & 15) == 0)
+    column_sums_kernel<4><<<unsigned((columns + 127) / 128), 32 * kSumLanes, 0, stream>>>(parts, count, columns, out, first, rest);
+  else
+    column_sums_kernel<1><<<unsigned((columns + 31) / 32), 32 * kSumLanes, 0, stream>>>(parts, count, columns, out, first, rest);
   MB200_CHECK_CUDA(cudaGetLastError());
   return kOk;
 }

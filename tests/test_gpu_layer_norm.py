@@ -45,6 +45,16 @@ def test_forward_and_gradients(rows, hidden, dtype):
     _check(x, dy, w.to(dtype), b.to(dtype))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,hidden", [(150, 264), (1001, 520), (300, 768), (601, 1024), (2500, 1032), (333, 2048), (1203, 129), (450, 1031)])
+def test_rows_side_by_side_in_a_block(rows, hidden, dtype):
+    """Rows of a few warps share a block in the backward pass: last blocks that are not full, rows that end inside a warp."""
+    g = _gen(rows * hidden)
+    x, dy = (torch.randn(rows, hidden, device=DEV, generator=g).to(dtype) for _ in range(2))
+    w, b = torch.randn(hidden, device=DEV, generator=g), torch.randn(hidden, device=DEV, generator=g)
+    _check(x, dy, w, b)
+
+
 @pytest.mark.parametrize("dtype", TYPES[:2])
 @pytest.mark.parametrize("which", ["both", "weight", "bias", "none"])
 @pytest.mark.parametrize("hidden", [96, 1001])
