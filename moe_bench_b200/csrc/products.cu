@@ -150,7 +150,7 @@ __device__ __forceinline__ Tile locate_tile(int tile, int part, const ProductArg
   return r;
 }
 
-// Both gradients: the input gradient's tiles, then the weight gradient's, so that only one wave of tiles is the last.
+// Both gradients: the input gradient's tiles, then the weight gradient's, so that one launch and one last wave of tiles do for both.
 template <int kKind>
 __device__ __forceinline__ Tile locate(int tile, int first_tiles, int part, const ProductArgs& p, const TileShape& s, const SmemTail* t) {
   if constexpr (kKind != kBothGrads) return locate_tile<kKind>(tile, part, p, s, t);
@@ -196,7 +196,7 @@ __device__ __forceinline__ void emit(const ProductArgs& p, const TileShape& shap
 // the pairs' order.  Called by all threads of the cluster; a cluster has one tile at most.
 template <int kKind, bool kFinish>
 __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape& shape, SmemTail* t, uint32_t ring, uint32_t tmem,
-                                           int worker, int part, uint32_t cta, int total_tiles, WaitCtx& ctx) {
+                                           int worker, int part, uint32_t cta, int total_tiles, int first_tiles, WaitCtx& ctx) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quarter = warp & 3, group = (warp - kFirstEpilogueWarp) >> 2;
   const bool mine = warp >= kFirstEpilogueWarp && worker < total_tiles;
@@ -204,7 +204,7 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
   Tile c{};
   bool ok = false;
   if (mine) {
-    c = locate_tile<kKind>(worker, part, p, shape, t);
+    c = locate<kKind>(worker, first_tiles, part, p, shape, t);
     ok = mbar_wait(smem_u32(&t->acc_full[0]), 0, ctx, 26);
     tc_fence_after();
   }
@@ -258,7 +258,7 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
         z[4 * i + 3] += from == part ? o[3] : q.w;
       }
     }
-    emit<kFinish>(p, shape, output_of(p, shape, 0), c, k, f, z, bias, res);
+    emit<kFinish>(p, shape, output_of(p, shape, kKind == kBothGrads && c.weight), c, k, f, z, bias, res);
   }
 }
 
@@ -351,13 +351,13 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     total_tiles = t->blocks[p.groups] * shape.f_tiles;
     half_rows = min(128, (t->max_len + 31) / 32 * 16);
   }
-  // a cluster that joins parts has one tile at most; only offsets that do not ascend could ask for more
-  if (shape.splits > 1) total_tiles = min(total_tiles, workers);
   const int first_tiles = total_tiles;
   if (kKind == kBothGrads) {
     total_tiles += p.groups * shape.row_blocks * shape.f_tiles;
     half_rows = max(half_rows, p.n <= 128 ? 64 : 128);
   }
+  // a cluster that joins parts has one tile at most; only offsets that do not ascend could ask for more
+  if (shape.splits > 1) total_tiles = min(total_tiles, workers);
   const int stage_bytes = kABytes + max(half_rows, 16) * 128;
   const int stages = min(kMaxStages, int(kRingBytes) / stage_bytes);
   tc_fence_before();
@@ -679,7 +679,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     }
   }
 
-  if (shape.splits > 1) join_parts<kKind, kFinish>(p, shape, t, ring, tmem, worker, part, cta, total_tiles, ctx);
+  if (shape.splits > 1) join_parts<kKind, kFinish>(p, shape, t, ring, tmem, worker, part, cta, total_tiles, first_tiles, ctx);
 
   // ---------------- teardown ----------------
   __syncwarp();
@@ -731,6 +731,7 @@ int active_clusters(const void* kernel, int splits, int device) {
 // Few tiles leave most pairs of CTAs idle: up to eight share a tile then, as long as all clusters run at the same time and
 // each pair has four steps.  `tiles`: as many as there can be.
 int split_count(const void* kernel, int64_t tiles, int64_t steps, int device) {
+  if (tiles * 2 > device_sm_count(device) / 2) return 1;  // the launch need not ask
   int s = int(std::min(int64_t(kMaxSplits), std::max(steps / 4, int64_t(1))));
   while (s > 1 && tiles > active_clusters(kernel, s, device)) --s;
   return s;
@@ -755,6 +756,18 @@ KernelFn kernel_of(ProductKind kind, bool finish) {
   }
 }
 
+int configure(ProductKind kind, bool finish, int device) {
+  const KernelFn kernel = kernel_of(kind, finish);
+  const int variant = kind == kForward ? (finish ? 1 : 0) : kind + 1;
+  static std::atomic<bool> configured[kMaxDevices][5];
+  if (device < 0 || device >= kMaxDevices || !configured[device][variant].load(std::memory_order_acquire)) {
+    MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)));
+    MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (device >= 0 && device < kMaxDevices) configured[device][variant].store(true, std::memory_order_release);
+  }
+  return kOk;
+}
+
 // Tiles that there can be.
 int64_t most_tiles(ProductKind kind, const ProductArgs& p) {
   const int64_t f_tiles = ceil_div(p.m, kTileFeatures);
@@ -762,6 +775,9 @@ int64_t most_tiles(ProductKind kind, const ProductArgs& p) {
   // a segment's last block may be short: at most one more per segment than the rows fill
   return (p.offsets ? int64_t(p.rows) / kTileRows + std::min(p.groups, p.rows) : ceil_div(p.rows, kTileRows)) * f_tiles;
 }
+
+// Steps of a tile's sum; of ragged segments in the weight gradient those of an average one.
+int64_t steps_of(ProductKind kind, const ProductArgs& p) { return ceil_div(kind == kWeightGrad ? p.rows / p.groups : p.k, kStep); }
 
 }  // namespace
 
@@ -803,23 +819,39 @@ int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaSt
   for (int i = weight ? 2 : 0; i < (weight ? 3 : kBoxes); ++i)
     if ((rc = make_map(&maps.b[i], args.b, weight ? args.n : args.k, args.rows, 1, args.b_pitch, 0, 16u << i, fp16))) return rc;
 
-  const int variant = kind == kForward ? (finish ? 1 : 0) : kind + 1;
   const KernelFn kernel = kernel_of(kind, finish);
-  static std::atomic<bool> configured[kMaxDevices][5];
-  if (device < 0 || device >= kMaxDevices || !configured[device][variant].load(std::memory_order_acquire)) {
-    MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)));
-    MB200_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    if (device >= 0 && device < kMaxDevices) configured[device][variant].store(true, std::memory_order_release);
-  }
-  // beyond half of the pairs nothing is split: the launch need not ask
-  s.splits = both || tiles * 2 > sms / 2
-                 ? 1
-                 : split_count(reinterpret_cast<const void*>(kernel), tiles, ceil_div(weight ? args.rows / args.groups : args.k, kStep), device);
+  if ((rc = configure(kind, finish, device))) return rc;
+  const int64_t steps = std::max(weight ? 0 : steps_of(kInputGrad, args), weight || both ? steps_of(kWeightGrad, args) : 0);
+  s.splits = split_count(reinterpret_cast<const void*>(kernel), tiles, steps, device);
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = cluster_config(int(std::min(tiles, int64_t(sms / 2))), s.splits, stream, attr);
   MB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps, args, s));
   return kOk;
 }
+
+namespace {
+
+// Whether both gradients take less time in one launch, by their steps (0.27 us): start, epilogue and launch are about 30, and
+// a launch's sums are as long as its longest tile's, split where it is, or as what the busiest pair of CTAs has to do.  1000 x 2048 ->
+// 1024: 12 us with one launch, 26 with two; 16384 x 7168 -> 256, 28 tiles of 256 steps after 1792 of 4: 140 and 127.
+bool one_launch(const ProductArgs& p, int device) {
+  const int64_t pairs = std::max(device_sm_count(device) / 2, 1);
+  const int64_t t1 = most_tiles(kInputGrad, p), s1 = steps_of(kInputGrad, p), t2 = most_tiles(kWeightGrad, p), s2 = steps_of(kWeightGrad, p);
+  auto time = [&](int64_t first, int64_t second) {
+    const int64_t longest = std::max(first ? s1 : 0, second ? s2 : 0);
+    const int splits = split_count(reinterpret_cast<const void*>(kernel_of(kBothGrads, false)), first + second, longest, device);
+    if (splits > 1) return 30 + ceil_div(longest, splits);
+    int64_t busiest = 0;
+    for (int64_t i = 0; i < pairs; ++i) {
+      const int64_t mine = ceil_div(std::max(first - i, int64_t(0)), pairs), all = ceil_div(std::max(first + second - i, int64_t(0)), pairs);
+      busiest = std::max(busiest, mine * s1 + (all - mine) * s2);
+    }
+    return 30 + busiest;
+  };
+  return time(t1, t2) <= time(t1, 0) + time(0, t2);
+}
+
+}  // namespace
 
 int launch_gradients(const ProductArgs& args, void* dx, void* dw, int dw_fp32, const void* w, int64_t w_pitch, int64_t w_group,
                      const void* x, int64_t x_pitch, int device, cudaStream_t stream) {
@@ -828,18 +860,23 @@ int launch_gradients(const ProductArgs& args, void* dx, void* dw, int dw_fp32, c
   p.a_pitch = w_pitch;
   p.a_group = w_group;
   p.epi.out = dx;
-  const int64_t pairs = device_sm_count(device) / 2;
-  // Dense: one launch for both, unless one has so few tiles that its sums are better split (4096 x 7168 -> 2048: 208 us
-  // with one, 231 with two).  Ragged segments: two, since reading all experts' weights and writing all their gradients at once
-  // takes longer than one after the other (32 experts of 1024 rows: 3.49 against 3.37 ms).
-  if (dx && dw && !p.offsets && most_tiles(kInputGrad, p) * 2 > pairs && most_tiles(kWeightGrad, p) * 2 > pairs) {
+  // One launch for both saves a last wave of tiles (dense, 4096 x 7168 -> 2048: 208 us, 231 with two) or all of a launch, unless
+  // the weights are so many that reading them and writing their gradients at once takes longer than one after the other (32
+  // experts of 2048 x 7168, 16384 rows: 1040 us, 920 with two; 256 of 2048 x 768, 8192 rows: the same; 16 of 7168 x 2048, 8192
+  // rows: 495, 530 with two).
+  int rc;
+  bool together = dx && dw && int64_t(p.groups) * p.n * p.m < int64_t(1) << 28;
+  if (together) {
+    if ((rc = configure(kBothGrads, false, device))) return rc;
+    together = one_launch(p, device);
+  }
+  if (together) {
     p.a2 = x;
     p.a2_pitch = x_pitch;
     p.out2 = dw;
     p.out2_fp32 = dw_fp32;
     return launch_product(kBothGrads, p, device, stream);
   }
-  int rc;
   if (dx && (rc = launch_product(kInputGrad, p, device, stream))) return rc;
   if (!dw) return kOk;
   p.a = x;

@@ -56,6 +56,21 @@ def test_products_and_gradients(sizes, k, n, dtype):
             assert not dw[i].any()
 
 
+@pytest.mark.parametrize("sizes,k,n", [([30, 0, 50, 20], 1024, 512), ([2000], 512, 300), ([0, 640, 1], 256, 1024), ([513, 0, 0, 255], 2048, 40),
+                                       ([100] * 16, 512, 256)])
+def test_gradients_where_pairs_share_tiles(sizes, k, n):
+    rows, e = sum(sizes), len(sizes)
+    g = _gen(rows * 7 + n)
+    x, w, dy = _normal(g, rows + 5, k), _normal(g, e, n, k, scale=k ** -0.5), _normal(g, rows + 5, n, scale=0.5)
+    x[:2], dy[:2], x[-3:], dy[-3:] = (float("nan"),) * 4  # outside the segments
+    keep = torch.full_like(x, 7.0)
+    dx, dw = capi.grouped_linear_backward(dy, x, w, _offsets(sizes, 2), dw_dtype=torch.float32, dx_out=keep)
+    (rx, bx), (rw, bw) = F.grouped_linear_backward(dy[2:-3], x[2:-3], w, sizes, torch.float32)
+    _good(dx[2:-3], (rx, bx), "dx")
+    _good(dw, (rw, bw), "dw")
+    assert (dx[:2] == 7).all() and (dx[-3:] == 7).all()
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_neighbours_and_rows_outside_have_no_part(bad):
     """NaN and inf in the rows of one expert, and in rows before, behind and between what counts, reach nobody else; rows

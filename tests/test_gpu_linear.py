@@ -90,6 +90,19 @@ def test_gradients(rows, k, n, dtype, with_slope):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("rows,k,n", [(20, 512, 512), (300, 1024, 1024), (130, 2048, 264), (600, 512, 333), (64, 4096, 64), (2000, 256, 1500),
+                                      (1000, 2048, 1024), (5000, 264, 72), (9000, 256, 520)])
+def test_both_gradients_with_sums_of_different_lengths(rows, k, n):
+    """In one launch or in two, split or not: dx sums over n, dw over the rows."""
+    g = _gen(rows + k)
+    x, w, dy = _normal(g, rows, k), _normal(g, n, k, scale=k ** -0.5), _normal(g, rows, n, scale=0.3)
+    ref = F.linear_backward(dy, x, w, None, torch.float32)
+    got = capi.linear_backward(dy, x, w, dw_dtype=torch.float32)
+    for name, a, b in zip(("dx", "dw", "db"), got, ref):
+        _good(a, b, name)
+    assert all(torch.equal(a, b) for a, b in zip(got, capi.linear_backward(dy, x, w, dw_dtype=torch.float32)))
+
+
 def test_fp32_output_gradient():
     g = _gen(5)
     x, w, dy = _normal(g, 65, 128), _normal(g, 48, 128, scale=0.1), torch.randn(65, 48, device=DEV, generator=g) * 1e-6
