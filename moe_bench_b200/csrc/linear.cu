@@ -20,7 +20,7 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // One pass over dy and slope, bound by HBM.  A block takes 32 * kVec columns of a run of rows, 8 rows side by side: a
 // thread has kVec neighbouring columns (16 bytes, or one element where rows do not start on vectors) of every eighth
 // row, four of them requested ahead, and sums them in fp32; the eight are added in order, and the runs' sums by
-// column_sums_kernel.  With slope 4096 x 2048 takes 10 us and 8192 x 7168 62 us with both kernels, 1.3 and 1.15 times its
+// column_sums_kernel, or where there are up to eight runs by the first block of a cluster.  With slope 4096 x 2048 takes 10 us and 8192 x 7168 62 us with both kernels, 1.3 and 1.15 times its
 // bytes at the copy rate (one element per thread in 64 runs: 22 and 236 us).
 constexpr int kRowLanes = 8;
 constexpr int kRowsAhead = 4;
@@ -33,6 +33,7 @@ struct OutputGrad {
   int64_t dy_pitch, dz_pitch;
   int rows, n, rows_per_chunk;
   int fp16;
+  int joined;          // the runs of a column are a cluster
 };
 
 // kVec elements as they lie in memory
@@ -110,9 +111,28 @@ __global__ void __launch_bounds__(256, 4) output_grad_kernel(const OutputGrad p)
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < kRowLanes; ++i) t += part[i][c];
-    p.sums[int64_t(blockIdx.y) * p.n + at] = t;
+    if (p.joined) part[0][c] = t;
+    else p.sums[int64_t(blockIdx.y) * p.n + at] = t;
   }
+  if (!p.joined) return;
+  cluster_sync();
+  if (blockIdx.y == 0)
+    for (int c = threadIdx.x; c < 32 * kVec; c += 256) {
+      const int at = int(blockIdx.x) * 32 * kVec + c;
+      if (at >= p.n) continue;
+      float t = 0.f;
+      for (int k = 0; k < int(gridDim.y); ++k) {
+        float v;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(smem_u32(&part[0][c]), k)) : "memory");
+        t += v;
+      }
+      p.sums[at] = t;
+    }
+  cluster_sync();  // the first block has read the others' sums
 }
+
+constexpr int kMostJoined = 8;      // runs that a cluster joins
+constexpr int kRowsJoined = 512;    // rows that are cut into so few runs
 
 struct GradLayout {
   int64_t dz_pitch, dz_bytes, sum_bytes;
@@ -126,10 +146,11 @@ GradLayout grad_layout(int64_t rows, int n, int device) {
   // eight blocks of 256 columns per SM, as long as each has 32 rows
   int64_t chunks = 8 * sms / ((n + 255) / 256);
   chunks = std::min(chunks, (rows + 31) / 32);
+  if (rows <= kRowsJoined) chunks = std::min(chunks, int64_t(kMostJoined));
   chunks = std::max(chunks, int64_t(1));
   l.rows_per_chunk = int((rows + chunks - 1) / chunks);
   l.chunks = l.rows_per_chunk > 0 ? int((rows + l.rows_per_chunk - 1) / l.rows_per_chunk) : 1;
-  l.sum_bytes = l.chunks > 1 ? round_up(int64_t(l.chunks) * n * 4, 256) : 0;
+  l.sum_bytes = l.chunks > kMostJoined ? round_up(int64_t(l.chunks) * n * 4, 256) : 0;
   return l;
 }
 
@@ -198,7 +219,8 @@ int prepare_output_grad(const void*& dy, int dy_fp32, int64_t& dy_pitch, const v
   g.dy = dy;
   g.slope = slope;
   g.dz = copy ? reinterpret_cast<uint16_t*>(ws) : nullptr;
-  g.sums = !db ? nullptr : l.chunks > 1 ? reinterpret_cast<float*>(ws + (copy ? l.dz_bytes : 0)) : db;
+  g.joined = db && l.chunks > 1 && l.chunks <= kMostJoined;
+  g.sums = !db ? nullptr : l.chunks > kMostJoined ? reinterpret_cast<float*>(ws + (copy ? l.dz_bytes : 0)) : db;
   g.dy_pitch = dy_pitch;
   g.dz_pitch = l.dz_pitch;
   g.rows = int(rows);
@@ -206,13 +228,20 @@ int prepare_output_grad(const void*& dy, int dy_fp32, int64_t& dy_pitch, const v
   g.rows_per_chunk = l.rows_per_chunk;
   g.fp16 = fp16;
   const bool vec = n % 8 == 0 && dy_pitch % 8 == 0 && aligned16(dy) && aligned16(slope);
-  const dim3 grid((n + (vec ? 255 : 31)) / (vec ? 256 : 32), l.chunks);
-  if (vec && dy_fp32) output_grad_kernel<8, true><<<grid, 256, 0, s>>>(g);
-  else if (vec) output_grad_kernel<8, false><<<grid, 256, 0, s>>>(g);
-  else if (dy_fp32) output_grad_kernel<1, true><<<grid, 256, 0, s>>>(g);
-  else output_grad_kernel<1, false><<<grid, 256, 0, s>>>(g);
-  MB200_CHECK_CUDA(cudaGetLastError());
-  if (db && l.chunks > 1) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.y = unsigned(l.chunks);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((n + (vec ? 255 : 31)) / (vec ? 256 : 32), l.chunks);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = g.joined ? 1 : 0;
+  const auto kernel = vec ? (dy_fp32 ? output_grad_kernel<8, true> : output_grad_kernel<8, false>)
+                          : (dy_fp32 ? output_grad_kernel<1, true> : output_grad_kernel<1, false>);
+  MB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, g));
+  if (db && l.chunks > kMostJoined) {
     if ((rc = launch_column_sums(g.sums, l.chunks, n, db, n, nullptr, s))) return rc;
   }
   uint16_t* dz = g.dz;
