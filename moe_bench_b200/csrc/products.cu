@@ -728,13 +728,16 @@ int active_clusters(const void* kernel, int splits, int device) {
   return n;
 }
 
-// Few tiles leave most pairs of CTAs idle: up to eight share a tile then, as long as all clusters run at the same time and
-// each pair has four steps.  `tiles`: as many as there can be.
+// Few tiles leave most pairs of CTAs idle: some share a tile then, as long as all clusters run at the same time.  The join
+// costs as much as 12 steps, whatever the number of pairs; with four (200 x 512 features: 24 steps 9.9 us instead of 11.5, two pairs
+// 11.4; 16 steps 9.5 and 9.6; 8 steps 9.0 and 7.6), more where each then still has 12 (64 steps 12.0 with five, 12.5 with four).
+// `tiles`: as many as there can be.
+constexpr int kJoinSteps = 12;
 int split_count(const void* kernel, int64_t tiles, int64_t steps, int device) {
   if (tiles * 2 > device_sm_count(device) / 2) return 1;  // the launch need not ask
-  int s = int(std::min(int64_t(kMaxSplits), std::max(steps / 4, int64_t(1))));
-  while (s > 1 && tiles > active_clusters(kernel, s, device)) --s;
-  return s;
+  int s = int(std::min(int64_t(kMaxSplits), std::max(steps / kJoinSteps, int64_t(4))));
+  while (s > 1 && steps - steps / s >= kJoinSteps && tiles > active_clusters(kernel, s, device)) --s;
+  return steps - steps / s >= kJoinSteps ? s : 1;
 }
 
 // Tiled view of 16-bit elements: c0 side by side, c1 `pitch` elements apart, c2 `group` elements apart.
@@ -840,7 +843,7 @@ bool one_launch(const ProductArgs& p, int device) {
   auto time = [&](int64_t first, int64_t second) {
     const int64_t longest = std::max(first ? s1 : 0, second ? s2 : 0);
     const int splits = split_count(reinterpret_cast<const void*>(kernel_of(kBothGrads, false)), first + second, longest, device);
-    if (splits > 1) return 30 + ceil_div(longest, splits);
+    if (splits > 1) return 30 + kJoinSteps + ceil_div(longest, splits);
     int64_t busiest = 0;
     for (int64_t i = 0; i < pairs; ++i) {
       const int64_t mine = ceil_div(std::max(first - i, int64_t(0)), pairs), all = ceil_div(std::max(first + second - i, int64_t(0)), pairs);
