@@ -138,20 +138,24 @@ struct GradLayout {
   int64_t dz_pitch, dz_bytes, sum_bytes;
   int chunks, rows_per_chunk;
 };
-GradLayout grad_layout(int64_t rows, int n, int device) {
+// `width`: columns of a block, 256 or (single elements) 32; runs of 256 columns are never fewer.
+GradLayout grad_layout(int64_t rows, int n, int width, int device) {
   const int sms = device_sm_count(device) > 0 ? device_sm_count(device) : 1;
   GradLayout l;
   l.dz_pitch = round_up(n, 8);
   l.dz_bytes = round_up(rows * l.dz_pitch * 2, 256);
-  // eight blocks of 256 columns per SM, as long as each has 32 rows
-  int64_t chunks = 8 * sms / ((n + 255) / 256);
-  chunks = std::min(chunks, (rows + 31) / 32);
+  // eight blocks per SM, as long as each has 32 rows (16384 x 515, single elements: 29 us with as many runs as 256 columns have)
+  int64_t chunks = 8 * sms / ((n + width - 1) / width);
   if (rows <= kRowsJoined) chunks = std::min(chunks, int64_t(kMostJoined));
   chunks = std::max(chunks, int64_t(1));
-  l.rows_per_chunk = int((rows + chunks - 1) / chunks);
+  constexpr int kTurn = kRowLanes * kRowsAhead;
+  l.rows_per_chunk = int(((rows + chunks - 1) / chunks + kTurn - 1) / kTurn * kTurn);
   l.chunks = l.rows_per_chunk > 0 ? int((rows + l.rows_per_chunk - 1) / l.rows_per_chunk) : 1;
   l.sum_bytes = l.chunks > kMostJoined ? round_up(int64_t(l.chunks) * n * 4, 256) : 0;
   return l;
+}
+bool grad_vectors(const void* dy, int64_t dy_pitch, const void* slope, int n) {
+  return n % 8 == 0 && dy_pitch % 8 == 0 && aligned16(dy) && aligned16(slope);
 }
 
 int check_precision(int precision, const char* what) {
@@ -199,7 +203,7 @@ int check_grad_workspace(const char* what, bool copy, bool sums, int64_t rows, i
                          int device, int64_t& need) {
   need = 0;
   if (!copy && !sums) return kOk;
-  const GradLayout l = grad_layout(rows, n, device);
+  const GradLayout l = grad_layout(rows, n, 256, device);
   need = (copy ? l.dz_bytes : 0) + (sums ? l.sum_bytes : 0);
   MB200_REQUIRE(need == 0 || (workspace && aligned16(workspace)), kInvalidArgument,
                 "%s: needs a 16-byte aligned workspace", what);
@@ -213,7 +217,8 @@ int prepare_output_grad(const void*& dy, int dy_fp32, int64_t& dy_pitch, const v
                         float* db, void* workspace, int device, cudaStream_t s) {
   int rc;
   if (!copy && !db) return kOk;
-  const GradLayout l = grad_layout(rows, n, device);
+  const bool vec = grad_vectors(dy, dy_pitch, slope, n);
+  const GradLayout l = grad_layout(rows, n, vec ? 256 : 32, device);
   char* ws = reinterpret_cast<char*>(workspace);
   OutputGrad g{};
   g.dy = dy;
@@ -227,7 +232,6 @@ int prepare_output_grad(const void*& dy, int dy_fp32, int64_t& dy_pitch, const v
   g.n = n;
   g.rows_per_chunk = l.rows_per_chunk;
   g.fp16 = fp16;
-  const bool vec = n % 8 == 0 && dy_pitch % 8 == 0 && aligned16(dy) && aligned16(slope);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
@@ -309,7 +313,7 @@ int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, co
 
 int64_t mb200_linear_backward_workspace_bytes(int64_t rows, int n, int copies_dy, int device) {
   if (check_sizes(rows, n, 8, "linear_backward_workspace_bytes")) return -1;
-  const GradLayout l = grad_layout(rows, n, device);
+  const GradLayout l = grad_layout(rows, n, 256, device);
   return (copies_dy ? l.dz_bytes : 0) + l.sum_bytes;
 }
 
@@ -387,7 +391,7 @@ int mb200_grouped_linear(int precision, const void* x, int64_t x_pitch, int64_t 
 
 int64_t mb200_grouped_linear_backward_workspace_bytes(int64_t rows, int n) {
   if (check_sizes(rows, n, 8, "grouped_linear_backward_workspace_bytes")) return -1;
-  return grad_layout(rows, n, 0).dz_bytes;
+  return grad_layout(rows, n, 256, 0).dz_bytes;
 }
 
 int mb200_grouped_linear_backward(int precision, const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch,
