@@ -191,6 +191,68 @@ __device__ __forceinline__ void emit(const ProductArgs& p, const TileShape& shap
   }
 }
 
+// Where rows do not start on vectors: one feature of 16 output rows per lane, as tensor memory has them, so that a warp's 32 single
+// elements lie side by side in a row.  The issue slots are the bound: types are told apart once per chunk, addresses run.
+struct ColumnResidual {
+  uint32_t v[8];
+};
+__device__ __forceinline__ ColumnResidual load_residual_column(const Epilogue& e, int m, const Tile& c, int chunk, int f) {
+  ColumnResidual r{};
+  if (e.residual && f < m) {
+    const int rows = c.valid - chunk * 16;
+    const uint16_t* at = reinterpret_cast<const uint16_t*>(e.residual) + (c.out_row + chunk * 16) * e.residual_pitch + f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i, at += e.residual_pitch)
+      if (i < rows) r.v[i / 2] |= uint32_t(*at) << 16 * (i & 1);
+  }
+  return r;
+}
+__device__ __forceinline__ void store_column(void* out, int fp32, int fp16, int64_t at, int m, int rows, const float (&z)[16]) {
+  if (fp32) {
+    float* to = reinterpret_cast<float*>(out) + at;
+#pragma unroll
+    for (int i = 0; i < 16; ++i, to += m)
+      if (i < rows) *to = z[i];
+  } else {
+    uint16_t* to = reinterpret_cast<uint16_t*>(out) + at;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const uint32_t h = pack_h16x2(z[i], z[i + 1], fp16);
+      if (i < rows) *to = uint16_t(h);
+      to += m;
+      if (i + 1 < rows) *to = uint16_t(h >> 16);
+      to += m;
+    }
+  }
+}
+template <bool kFinish>
+__device__ __forceinline__ void emit_column(const ProductArgs& p, const Output& out, const Tile& c, int chunk, int f, float (&z)[16],
+                                            float bias, const ColumnResidual& res) {
+  const Epilogue& e = p.epi;
+  if (f >= p.m) return;
+  const int rows = c.valid - chunk * 16;
+  const int64_t at = (c.out_row + chunk * 16) * p.m + f;
+  if (kFinish) {
+    float slope[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] += bias;
+    if (e.slope) {
+      activate<true>(e.act, z, slope);
+      store_column(e.slope, 0, e.fp16, at, p.m, rows, slope);
+    } else if (e.act) {
+      activate<false>(e.act, z, slope);
+    }
+    if (e.residual)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) z[i] += load_h16(&res.v[i / 2], i & 1, e.fp16);
+  }
+  store_column(out.ptr, out.fp32, e.fp16, at, p.m, rows, z);
+}
+__device__ __forceinline__ float load_bias(const Epilogue& e, int m, int f) {
+  if (e.bias == nullptr || f >= m) return 0.f;
+  return e.bias_fp32 ? __ldg(reinterpret_cast<const float*>(e.bias) + f) : load_h16(e.bias, f, e.fp16);
+}
+
 // The pairs of a cluster have a part of the same tile's sums each, in tensor memory.  Pair k finishes the chunks
 // k, k + splits, ...: it gets the other pairs' parts of them pushed into its ring, which nothing uses any more, and adds them in
 // the pairs' order.  Called by all threads of the cluster; a cluster has one tile at most.
@@ -234,6 +296,30 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
   __syncwarp();
   cluster_sync();
   if (!ok) return;
+  const Output out = output_of(p, shape, kKind == kBothGrads && c.weight);
+  if (!out.vec) {
+    const int f = c.f0 + int(cta & 1) * 128 + quarter * 32 + lane;
+    const float bias = kFinish ? load_bias(p.epi, p.m, f) : 0.f;
+    for (int k = part + group * splits; k < chunks; k += 2 * splits) {
+      ColumnResidual res{};
+      if (kFinish) res = load_residual_column(p.epi, p.m, c, k, f);
+      uint32_t v[16];
+      tmem_ld16(lanes + k * 16, v);
+      tmem_ld_wait16(v);
+      float z[16] = {};
+      for (int from = 0; from < splits; ++from) {
+        const uint32_t at = ring + block_of(k, from) + lane * 4;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float q;
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(q) : "r"(at + i * 128) : "memory");
+          z[i] += from != part ? q : summed ? __uint_as_float(v[i]) : 0.f;
+        }
+      }
+      emit_column<kFinish>(p, out, c, k, f, z, bias, res);
+    }
+    return;
+  }
   const int f = c.f0 + int(cta & 1) * 128 + quarter * 32 + 4 * (lane & 7);
   Bias4 bias{};
   if (kFinish) bias = load_bias4(p.epi, p.m, f);
@@ -258,7 +344,7 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
         z[4 * i + 3] += from == part ? o[3] : q.w;
       }
     }
-    emit<kFinish>(p, shape, output_of(p, shape, kKind == kBothGrads && c.weight), c, k, f, z, bias, res);
+    emit<kFinish>(p, shape, out, c, k, f, z, bias, res);
   }
 }
 
@@ -652,6 +738,23 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
 #pragma unroll
           for (int u = 0; u < 2; ++u) place(u, z[u]);
           store(out.ptr, k);
+        }
+      } else if (!out.vec) {
+        const int f1 = c.f0 + int(rank) * 128 + quarter * 32 + lane;
+        const float bias1 = kFinish ? load_bias(p.epi, p.m, f1) : 0.f;
+        if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
+        tc_fence_after();
+        for (int k = first_chunk; k < chunks; k += 2) {
+          ColumnResidual res{};
+          if (kFinish) res = load_residual_column(p.epi, p.m, c, k, f1);
+          uint32_t v[16];
+          tmem_ld16(lanes + k * 16, v);
+          tmem_ld_wait16(v);
+          if (k + 2 >= chunks) release();
+          float z[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) z[i] = summed ? __uint_as_float(v[i]) : 0.f;
+          emit_column<kFinish>(p, out, c, k, f1, z, bias1, res);
         }
       } else {
         // a chunk's share of the residual is requested one chunk ahead
