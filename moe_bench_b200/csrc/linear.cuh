@@ -68,6 +68,31 @@ __device__ __forceinline__ float load_h16(const void* p, int64_t i, int fp16) {
 // rounding and about 2 units of an fp32 output.
 __device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 
+// The normal distribution's mass beyond |z|, 1 - Phi(|z|), over exp(-z^2 / 2): u P(u) with u = 1 / (1 + 0.28 |z|), where P is a
+// polynomial fitted to it (relative error at most 1.7e-7 for all z, by reweighted least squares), so that the mass keeps
+// its digits however small it is.  GELU and its derivative need that exponential anyway: with the library's erfc on top of
+// it 8192 x 2048 -> 7168 took 233 us, 260 with the slope, 163 without an activation.
+template <int kCount>
+__device__ __forceinline__ void gelu_tail(const float (&z)[kCount], float (&out)[kCount]) {
+  constexpr float kP[9] = {0.11170385777950287f, 0.11169980466365814f,   0.10308467596769333f, 0.08363072574138641f, 0.07277529686689377f,
+                           -0.006449869368225336f, 0.0924290269613266f, -0.09359373897314072f, 0.024720141664147377f};
+#pragma unroll
+  for (int i = 0; i < kCount; i += 2) {
+    const float a = __fdividef(1.f, fmaf(0.28f, fabsf(z[i]), 1.f)), b = __fdividef(1.f, fmaf(0.28f, fabsf(z[i + 1]), 1.f));
+    const uint64_t u = pack_f32x2(__float_as_uint(a), __float_as_uint(b));
+    uint64_t p = pack_f32x2(__float_as_uint(kP[8]), __float_as_uint(kP[8]));
+#pragma unroll
+    for (int k = 7; k >= 0; --k) {
+      uint64_t next = pack_f32x2(__float_as_uint(kP[k]), __float_as_uint(kP[k]));
+      fma_f32x2(next, p, u);
+      p = next;
+    }
+    unpack_f32x2(p, out[i], out[i + 1]);
+    out[i] *= a;
+    out[i + 1] *= b;
+  }
+}
+
 // act(z) in place, and with kSlope act'(z), for values that have nothing to do with one another.  Both stay finite
 // wherever z is; NaN stays NaN in act(z).
 template <bool kSlope, int kCount>
@@ -88,15 +113,19 @@ __device__ __forceinline__ void activate(int act, float (&z)[kCount], float (&sl
         z[i] *= s;
       }
       break;
-    case kActGelu:
+    case kActGelu: {
+      float tail[kCount];
+      gelu_tail(z, tail);
 #pragma unroll
       for (int i = 0; i < kCount; ++i) {
-        // (1 + erf(z / sqrt 2)) / 2 by the complement: the sum cancels below 0
-        const float c = 0.5f * erfcf(-z[i] * 0.70710678118654752f);
-        if (kSlope) slope[i] = c + z[i] * (__expf(-0.5f * z[i] * z[i]) * 0.39894228040143268f);
+        const float e = __expf(-0.5f * z[i] * z[i]);
+        const float q = tail[i] * e;
+        const float c = z[i] > 0.f ? 1.f - q : q;
+        if (kSlope) slope[i] = c + z[i] * (e * 0.39894228040143268f);
         z[i] *= c;
       }
       break;
+    }
     case kActGeluTanh:
 #pragma unroll
       for (int i = 0; i < kCount; ++i) {
