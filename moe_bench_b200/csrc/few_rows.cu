@@ -43,6 +43,58 @@ __device__ __forceinline__ void mma_h16(float (&d)[4], uint32_t a0, uint32_t a1,
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The epilogue of four neighbouring features of a row; `vec`: every tensor takes them as one access (then m is a multiple of 4).
+// The residual may be the output's buffer: its loads promise nothing, and come before the row's stores.
+__device__ __forceinline__ void store4(void* out, int fp32, int fp16, int m, int64_t row, int f, const float (&v)[4], int vec) {
+  const int64_t at = row * m + f;
+  if (vec) {
+    if (fp32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + at) =
+        make_uint2(pack_h16x2(v[0], v[1], fp16), pack_h16x2(v[2], v[3], fp16));
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (f + k < m) {
+      if (fp32) reinterpret_cast<float*>(out)[at + k] = v[k];
+      else reinterpret_cast<uint16_t*>(out)[at + k] = to_h16(v[k], fp16);
+    }
+}
+__device__ __forceinline__ void finish4(const Epilogue& e, int m, int64_t row, int f, float (&z)[4], int vec) {
+  if (e.bias)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (f + i < m) z[i] += e.bias_fp32 ? __ldg(reinterpret_cast<const float*>(e.bias) + f + i) : load_h16(e.bias, f + i, e.fp16);
+  float residual[4] = {};
+  if (e.residual) {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(e.residual) + row * e.residual_pitch + f;
+    if (vec) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) residual[i] = load_h16(&v, i, e.fp16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (f + i < m) residual[i] = load_h16(p, i, e.fp16);
+    }
+  }
+  float slope[4];
+  if (e.slope) {
+    activate<true>(e.act, z, slope);
+    store4(e.slope, 0, e.fp16, m, row, f, slope, vec);
+  } else if (e.act) {
+    activate<false>(e.act, z, slope);
+  }
+  if (e.residual)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] += residual[i];
+  store4(e.out, e.out_fp32, e.fp16, m, row, f, z, vec);
+}
+int epilogue_vec(const Epilogue& e, int m) {
+  auto at = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
+  return m % 4 == 0 && at(e.out, e.out_fp32 ? 16 : 8) && at(e.slope, 8) && (!e.residual || (at(e.residual, 8) && e.residual_pitch % 4 == 0));
+}
+
 // kOctets: groups of 8 rows
 template <int kOctets>
 __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const ProductArgs p, int parts, int vec) {
@@ -113,8 +165,7 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const ProductArgs
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[e] += v[e];
       }
-      finish4<1>(p.epi, p.m, row, 1, row + 1, f0 + f, z, load_bias4(p.epi, p.m, f0 + f),
-                 load_residual4<1>(p.epi, p.m, row, 1, row + 1, f0 + f, vec), vec);
+      finish4(p.epi, p.m, row, f0 + f, z, vec);
     }
   }
   if (parts > 1) cluster_sync();  // the other blocks' sums have been read

@@ -142,94 +142,6 @@ __device__ __forceinline__ void activate(int act, float (&z)[kCount], float (&sl
   }
 }
 
-struct Bias4 {
-  float v[4];
-};
-__device__ __forceinline__ Bias4 load_bias4(const Epilogue& e, int m, int f) {
-  Bias4 b{};
-  if (e.bias)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (f + i < m) b.v[i] = e.bias_fp32 ? __ldg(reinterpret_cast<const float*>(e.bias) + f + i) : load_h16(e.bias, f + i, e.fp16);
-  return b;
-}
-// kRows output rows, `step` apart, x four features side by side; rows from `last` on and features from m on do not exist.
-// `vec`: every tensor takes four features as one access (then m is a multiple of 4).
-// The residual may be the output's buffer: its loads promise nothing, and come before the rows' stores.
-template <int kRows>
-struct Residual4 {
-  uint2 v[kRows];
-};
-template <int kRows>
-__device__ __forceinline__ Residual4<kRows> load_residual4(const Epilogue& e, int m, int64_t row, int step, int64_t last, int f, bool vec) {
-  Residual4<kRows> r{};
-  if (e.residual) {
-    const uint16_t* at = reinterpret_cast<const uint16_t*>(e.residual) + f;
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-      if (row + i * step < last) {
-        const uint16_t* p = at + (row + i * step) * e.residual_pitch;
-        if (vec) {
-          if (f < m) r.v[i] = *reinterpret_cast<const uint2*>(p);
-        } else {
-          uint16_t h[4] = {};
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (f + k < m) h[k] = p[k];
-          r.v[i] = make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
-        }
-      }
-  }
-  return r;
-}
-
-__device__ __forceinline__ void store4(void* out, int fp32, int fp16, int m, int64_t row, int f, const float* v, bool vec) {
-  if (f >= m) return;
-  const int64_t at = row * m + f;
-  if (vec) {
-    if (fp32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-    else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + at) =
-        make_uint2(pack_h16x2(v[0], v[1], fp16), pack_h16x2(v[2], v[3], fp16));
-    return;
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (f + k < m) {
-      if (fp32) reinterpret_cast<float*>(out)[at + k] = v[k];
-      else reinterpret_cast<uint16_t*>(out)[at + k] = to_h16(v[k], fp16);
-    }
-}
-
-template <int kRows>
-__device__ __forceinline__ void finish4(const Epilogue& e, int m, int64_t row, int step, int64_t last, int f, float (&z)[4 * kRows],
-                                        const Bias4& bias, const Residual4<kRows>& res, bool vec) {
-  float slope[4 * kRows];
-#pragma unroll
-  for (int i = 0; i < 4 * kRows; ++i) z[i] += bias.v[i & 3];
-  if (e.slope) {
-    activate<true>(e.act, z, slope);
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-      if (row + i * step < last) store4(e.slope, 0, e.fp16, m, row + i * step, f, slope + 4 * i, vec);
-  } else if (e.act) {
-    activate<false>(e.act, z, slope);
-  }
-  if (e.residual)
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) z[4 * i + k] += load_h16(&res.v[i], k, e.fp16);
-#pragma unroll
-  for (int i = 0; i < kRows; ++i)
-    if (row + i * step < last) store4(e.out, e.out_fp32, e.fp16, m, row + i * step, f, z + 4 * i, vec);
-}
-
-// Whether the epilogue can access four neighbouring features of every tensor at once.
-inline int epilogue_vec(const Epilogue& e, int m) {
-  auto at = [](const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
-  return m % 4 == 0 && at(e.out, e.out_fp32 ? 16 : 8) && at(e.slope, 8) && (!e.residual || (at(e.residual, 8) && e.residual_pitch % 4 == 0));
-}
-
 // The memory that a call writes must be apart from all other memory it is given: a kernel reads its inputs while it writes.
 struct Span {
   const char* name;

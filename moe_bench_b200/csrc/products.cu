@@ -17,8 +17,8 @@
 // 384 threads: warp 0 loads, warp 1 of the pair's first CTA issues the products, warp 2 clears those tails,
 // warps 4-11 drain the accumulators (two sets, so that the next tile's products run meanwhile).  A lane holds one
 // feature of many output rows, memory wants many features of one row: where outputs are of 16 bits and start on 16 bytes, 32
-// features x 32 output rows at a time are read as fragments, finished, rounded and transposed by stmatrix; else 32 x 16
-// go through a 2 KiB block of shared memory still in fp32.  Every wait is bounded.
+// features x 32 output rows at a time are read as fragments, finished, rounded and transposed by stmatrix; else a warp
+// stores its lanes' features row by row.  Every wait is bounded.
 //
 // Few tiles leave pairs idle, so up to eight pairs form a cluster and share a tile, each with a part of its sums; the parts
 // meet in shared memory and are added in the pairs' order (join_parts).
@@ -74,9 +74,8 @@ struct TileShape {
   int f_tiles;      // feature blocks
   int row_blocks;   // weight gradient: blocks of output rows per group
   int splits;       // pairs of CTAs that share a tile, each with a part of its sums; they form a cluster
-  int vec;          // the epilogue may access four features at once
-  int vec2, vec8_2; // the same two for the weight gradient where both gradients are computed
   int vec8;         // the output is of 16 bits, and every tensor takes eight features as one access
+  int vec8_2;       // the same for the weight gradient where both gradients are computed
 };
 
 __device__ int g_status[1];  // first failure of a wait
@@ -170,29 +169,17 @@ __device__ __forceinline__ void turn_chunk(float* block, const uint32_t (&v)[16]
   __syncwarp();
 }
 
-// Such a chunk through the epilogue.
 struct Output {
   void* ptr;
-  int fp32, vec, vec8;
+  int fp32, vec8;
 };
 __device__ __forceinline__ Output output_of(const ProductArgs& p, const TileShape& s, int both_and_weight) {
-  return both_and_weight ? Output{p.out2, p.out2_fp32, s.vec2, s.vec8_2} : Output{p.epi.out, p.epi.out_fp32, s.vec, s.vec8};
-}
-template <bool kFinish>
-__device__ __forceinline__ void emit(const ProductArgs& p, const TileShape& shape, const Output& out, const Tile& c, int chunk, int f,
-                                     float (&z)[16], const Bias4& bias, const Residual4<4>& res) {
-  const int64_t row = c.out_row + chunk * 16 + ((threadIdx.x & 31) >> 3), last = c.out_row + c.valid;
-  if (kFinish) {
-    finish4<4>(p.epi, p.m, row, 4, last, f, z, bias, res, shape.vec);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (row + 4 * i < last) store4(out.ptr, out.fp32, p.epi.fp16, p.m, row + 4 * i, f, z + 4 * i, out.vec);
-  }
+  return both_and_weight ? Output{p.out2, p.out2_fp32, s.vec8_2} : Output{p.epi.out, p.epi.out_fp32, s.vec8};
 }
 
-// Where rows do not start on vectors: one feature of 16 output rows per lane, as tensor memory has them, so that a warp's 32 single
-// elements lie side by side in a row.  The issue slots are the bound: types are told apart once per chunk, addresses run.
+// fp32 outputs, rows that do not start on vectors and joined parts: one feature of 16 output rows per lane, as tensor memory has
+// them, so that a warp's 32 single elements lie side by side in a row.  The issue slots are the bound: types are told apart
+// once per chunk, addresses run (7619 x 72 -> 515, bf16: 11.8 us; 20.8 with four features of a row per lane).
 struct ColumnResidual {
   uint32_t v[8];
 };
@@ -297,54 +284,25 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
   cluster_sync();
   if (!ok) return;
   const Output out = output_of(p, shape, kKind == kBothGrads && c.weight);
-  if (!out.vec) {
-    const int f = c.f0 + int(cta & 1) * 128 + quarter * 32 + lane;
-    const float bias = kFinish ? load_bias(p.epi, p.m, f) : 0.f;
-    for (int k = part + group * splits; k < chunks; k += 2 * splits) {
-      ColumnResidual res{};
-      if (kFinish) res = load_residual_column(p.epi, p.m, c, k, f);
-      uint32_t v[16];
-      tmem_ld16(lanes + k * 16, v);
-      tmem_ld_wait16(v);
-      float z[16] = {};
-      for (int from = 0; from < splits; ++from) {
-        const uint32_t at = ring + block_of(k, from) + lane * 4;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float q;
-          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(q) : "r"(at + i * 128) : "memory");
-          z[i] += from != part ? q : summed ? __uint_as_float(v[i]) : 0.f;
-        }
-      }
-      emit_column<kFinish>(p, out, c, k, f, z, bias, res);
-    }
-    return;
-  }
-  const int f = c.f0 + int(cta & 1) * 128 + quarter * 32 + 4 * (lane & 7);
-  Bias4 bias{};
-  if (kFinish) bias = load_bias4(p.epi, p.m, f);
+  const int f = c.f0 + int(cta & 1) * 128 + quarter * 32 + lane;
+  const float bias = kFinish ? load_bias(p.epi, p.m, f) : 0.f;
   for (int k = part + group * splits; k < chunks; k += 2 * splits) {
-    Residual4<4> res{};
-    if (kFinish) res = load_residual4<4>(p.epi, p.m, c.out_row + k * 16 + (lane >> 3), 4, c.out_row + c.valid, f, shape.vec);
+    ColumnResidual res{};
+    if (kFinish) res = load_residual_column(p.epi, p.m, c, k, f);
     uint32_t v[16];
     tmem_ld16(lanes + k * 16, v);
     tmem_ld_wait16(v);
-    float own[16], z[16] = {};
-    turn_chunk(t->turn[warp - kFirstEpilogueWarp], v, summed, own);
+    float z[16] = {};
     for (int from = 0; from < splits; ++from) {
-      const uint32_t at = ring + block_of(k, from) + (lane >> 3) * 128 + (lane & 7) * 16;
+      const uint32_t at = ring + block_of(k, from) + lane * 4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float4 q;
-        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w) : "r"(at + i * 512) : "memory");
-        const float* o = own + 4 * i;
-        z[4 * i] += from == part ? o[0] : q.x;
-        z[4 * i + 1] += from == part ? o[1] : q.y;
-        z[4 * i + 2] += from == part ? o[2] : q.z;
-        z[4 * i + 3] += from == part ? o[3] : q.w;
+      for (int i = 0; i < 16; ++i) {
+        float q;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(q) : "r"(at + i * 128) : "memory");
+        z[i] += from != part ? q : summed ? __uint_as_float(v[i]) : 0.f;
       }
     }
-    emit<kFinish>(p, shape, out, c, k, f, z, bias, res);
+    emit_column<kFinish>(p, out, c, k, f, z, bias, res);
   }
 }
 
@@ -609,9 +567,6 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
       const Tile c = locate<kKind>(tile, first_tiles, part, p, shape, t);
       const Output out = output_of(p, shape, kKind == kBothGrads && c.weight);
       const uint32_t buf = it & 1, use = it >> 1;
-      const int f = c.f0 + int(rank) * 128 + quarter * 32 + 4 * (lane & 7);
-      Bias4 bias{};
-      if (kFinish) bias = load_bias4(p.epi, p.m, f);
       const bool summed = c.step1 > c.step0;
       const uint32_t lanes = tmem + buf * 256 + (uint32_t(quarter * 32) << 16);
       const int chunks = (c.valid + 15) >> 4;
@@ -739,42 +694,33 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
           for (int u = 0; u < 2; ++u) place(u, z[u]);
           store(out.ptr, k);
         }
-      } else if (!out.vec) {
-        const int f1 = c.f0 + int(rank) * 128 + quarter * 32 + lane;
-        const float bias1 = kFinish ? load_bias(p.epi, p.m, f1) : 0.f;
+      } else if (!kFinish && out.vec8) {
+        // a weight gradient without rows is 0
+        if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
+        tc_fence_after();
+        release();
+        const int f8 = c.f0 + int(rank) * 128 + quarter * 32 + (lane & 3) * 8;
+        for (int r = first_chunk * 8 + (lane >> 2); r < c.valid; r += 16)
+          if (f8 < p.m)
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out.ptr) + (c.out_row + r) * p.m + f8) = make_uint4(0, 0, 0, 0);
+      } else {
+        const int f = c.f0 + int(rank) * 128 + quarter * 32 + lane;
+        const float bias = kFinish ? load_bias(p.epi, p.m, f) : 0.f;
+        ColumnResidual res{};  // a chunk ahead
+        if (kFinish) res = load_residual_column(p.epi, p.m, c, first_chunk, f);
         if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
         tc_fence_after();
         for (int k = first_chunk; k < chunks; k += 2) {
-          ColumnResidual res{};
-          if (kFinish) res = load_residual_column(p.epi, p.m, c, k, f1);
           uint32_t v[16];
           tmem_ld16(lanes + k * 16, v);
+          ColumnResidual next{};
+          if (kFinish) next = load_residual_column(p.epi, p.m, c, k + 2, f);
           tmem_ld_wait16(v);
           if (k + 2 >= chunks) release();
           float z[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) z[i] = summed ? __uint_as_float(v[i]) : 0.f;
-          emit_column<kFinish>(p, out, c, k, f1, z, bias1, res);
-        }
-      } else {
-        // a chunk's share of the residual is requested one chunk ahead
-        Residual4<4> res{};
-        const int64_t last = c.out_row + c.valid;
-        if (kFinish && first_chunk < chunks)
-          res = load_residual4<4>(p.epi, p.m, c.out_row + first_chunk * 16 + (lane >> 3), 4, last, f, shape.vec);
-        if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
-        tc_fence_after();
-        for (int k = first_chunk; k < chunks; k += 2) {
-          uint32_t v[16];
-          tmem_ld16(lanes + k * 16, v);
-          Residual4<4> next{};
-          if (kFinish && k + 2 < chunks)
-            next = load_residual4<4>(p.epi, p.m, c.out_row + (k + 2) * 16 + (lane >> 3), 4, last, f, shape.vec);
-          tmem_ld_wait16(v);
-          if (k + 2 >= chunks) release();
-          float z[16];
-          turn_chunk(turn_block, v, summed, z);
-          emit<kFinish>(p, shape, out, c, k, f, z, bias, res);
+          emit_column<kFinish>(p, out, c, k, f, z, bias, res);
           res = next;
         }
       }
@@ -907,10 +853,8 @@ int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaSt
                 (long long)tiles);
   const Epilogue& e = args.epi;
   const bool finish = e.bias || e.act || e.residual || e.slope;
-  s.vec = epilogue_vec(e, args.m);
   s.vec8 = !e.out_fp32 && args.m % 8 == 0 && aligned_to(e.out, 16) && aligned_to(e.slope, 16) &&
            (!e.residual || (aligned_to(e.residual, 16) && e.residual_pitch % 8 == 0));
-  s.vec2 = args.m % 4 == 0 && aligned_to(args.out2, args.out2_fp32 ? 16 : 8);
   s.vec8_2 = !args.out2_fp32 && args.m % 8 == 0 && aligned_to(args.out2, 16);
 
   Maps maps{};
