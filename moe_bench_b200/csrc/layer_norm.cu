@@ -5,8 +5,9 @@
 //
 // Statistics, gradients of the parameters and everything in between are fp32; y and dx are rounded once.
 //
-// Bound by HBM: bf16 rows of 7168 run at 5.7 TB/s forward (32768 of them 165 us, 143 at the copy rate) and at 5.5 backward (257
-// of 215 us); what is missing is the exchange within a row, which has 14 warps on an SM to hide behind.  8 rows take 4 us.
+// Bound by HBM: bf16 rows of 7168 run at 5.7 TB/s forward (32768 of them 165 us, 143 at the copy rate) and at 5.1 backward (16384
+// of them 139 us, 108 at the copy rate); what is missing is the exchange within a row, which has 14 warps on an SM to hide
+// behind.  8 rows take 3.7 us forward and 7.8 backward, half of that the second kernel.
 
 #include <algorithm>
 #include <atomic>
