@@ -76,6 +76,7 @@ struct TileShape {
   int splits;       // pairs of CTAs that share a tile, each with a part of its sums; they form a cluster
   int vec8;         // the output is of 16 bits, and every tensor takes eight features as one access
   int vec8_2;       // the same for the weight gradient where both gradients are computed
+  int rounds, lead; // dense gradients in one launch: see Walk; rounds -1: one tile after the other
 };
 
 __device__ int g_status[1];  // first failure of a wait
@@ -149,7 +150,7 @@ __device__ __forceinline__ Tile locate_tile(int tile, int part, const ProductArg
   return r;
 }
 
-// Both gradients: the input gradient's tiles, then the weight gradient's, so that one launch and one last wave of tiles do for both.
+// Both gradients: the input gradient's tiles have the first numbers, then come the weight gradient's.
 template <int kKind>
 __device__ __forceinline__ Tile locate(int tile, int first_tiles, int part, const ProductArgs& p, const TileShape& s, const SmemTail* t) {
   if constexpr (kKind != kBothGrads) return locate_tile<kKind>(tile, part, p, s, t);
@@ -168,6 +169,33 @@ __device__ __forceinline__ void turn_chunk(float* block, const uint32_t (&v)[16]
       *reinterpret_cast<const float4*>(block + ((lane >> 3) + 4 * i) * 32 + 4 * (lane & 7));
   __syncwarp();
 }
+
+// The tiles of a pair (or, with shared tiles, of a cluster: its only one), in turn.  Dense gradients: first tiles of the input
+// gradient, then of the weight gradient, whose sums may be long.  Where the latter do not come out even, the first `lead` pairs have one
+// more of them, and of the former only `rounds`; the others go on alone (9000 x 7168 -> 256, 28 tiles of 141 steps after 1008 of 4: 95
+// us in order, 76 so).
+template <int kKind>
+struct Walk {
+  int tile;  // from `total` on there is none
+  int first, total, worker, workers, lead, rounds, round;
+  __device__ __forceinline__ Walk(int first_, int total_, int worker_, int workers_, const TileShape& s)
+      : tile(worker_), first(first_), total(total_), worker(worker_), workers(workers_), lead(s.lead), rounds(s.rounds), round(0) {
+    if (kKind == kBothGrads && rounds >= 0) at_round();
+  }
+  __device__ __forceinline__ void at_round() {
+    // tile numbers stay below 2^30, and no round starts far behind the last
+    const int t = round < rounds ? round * workers + worker : rounds * workers + (round - rounds) * (workers - lead) + worker - lead;
+    tile = t < first && (worker >= lead || round < rounds) ? t : first + worker;
+  }
+  __device__ __forceinline__ void next() {
+    if (kKind != kBothGrads || rounds < 0 || tile >= first) {
+      tile += workers;
+    } else {
+      ++round;
+      at_round();
+    }
+  }
+};
 
 struct Output {
   void* ptr;
@@ -419,8 +447,8 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     // step's 520).  The ring's first round finds every stage empty.
     int stage = 0, round = 0;
     bool ok = true;
-    for (int tile = worker; ok && tile < total_tiles; tile += workers) {
-      const Tile c = locate<kKind>(tile, first_tiles, part, p, shape, t);
+    for (Walk<kKind> walk(first_tiles, total_tiles, worker, workers, shape); ok && walk.tile < total_tiles; walk.next()) {
+      const Tile c = locate<kKind>(walk.tile, first_tiles, part, p, shape, t);
       const int steps = c.step1 - c.step0;
       if (elect_one()) {
         const int half = c.cols >> 1;
@@ -484,8 +512,8 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     uint32_t it = 0;
     bool ok = true;
     const uint32_t fmt = p.epi.fp16 ? 0u : 1u;
-    for (int tile = worker; rank == 0 && ok && tile < total_tiles; tile += workers, ++it) {
-      const Tile c = locate<kKind>(tile, first_tiles, part, p, shape, t);
+    for (Walk<kKind> walk(first_tiles, total_tiles, worker, workers, shape); rank == 0 && ok && walk.tile < total_tiles; walk.next(), ++it) {
+      const Tile c = locate<kKind>(walk.tile, first_tiles, part, p, shape, t);
       const int steps = c.step1 - c.step0;
       if (elect_one()) {
         const uint32_t buf = it & 1, use = it >> 1;
@@ -535,8 +563,8 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     int stage = 0;
     uint32_t phases = 0;  // parity of raw[stage], one bit each
     bool ok = true;
-    for (int tile = worker; kKind >= kWeightGrad && ok && tile < total_tiles; tile += workers) {
-      const Tile c = locate<kKind>(tile, first_tiles, part, p, shape, t);
+    for (Walk<kKind> walk(first_tiles, total_tiles, worker, workers, shape); kKind >= kWeightGrad && ok && walk.tile < total_tiles; walk.next()) {
+      const Tile c = locate<kKind>(walk.tile, first_tiles, part, p, shape, t);
       const int last = c.depth / kStep;
       if ((kKind == kWeightGrad || c.weight) && c.depth % kStep != 0 && last >= c.step0 && last < c.step1) {
         const int at = (stage + last - c.step0) % stages;
@@ -563,8 +591,8 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
     // ---------------- epilogue: each warp on 32 features ----------------
     float* turn_block = t->turn[warp - kFirstEpilogueWarp];
     uint32_t it = 0;
-    for (int tile = worker; tile < total_tiles; tile += workers, ++it) {
-      const Tile c = locate<kKind>(tile, first_tiles, part, p, shape, t);
+    for (Walk<kKind> walk(first_tiles, total_tiles, worker, workers, shape); walk.tile < total_tiles; walk.next(), ++it) {
+      const Tile c = locate<kKind>(walk.tile, first_tiles, part, p, shape, t);
       const Output out = output_of(p, shape, kKind == kBothGrads && c.weight);
       const uint32_t buf = it & 1, use = it >> 1;
       const bool summed = c.step1 > c.step0;
@@ -831,6 +859,48 @@ int64_t most_tiles(ProductKind kind, const ProductArgs& p) {
 // Steps of a tile's sum; of ragged segments in the weight gradient those of an average one.
 int64_t steps_of(ProductKind kind, const ProductArgs& p) { return ceil_div(kind == kWeightGrad ? p.rows / p.groups : p.k, kStep); }
 
+// Time of a launch in steps (0.27 us), start, epilogue of the last tile and launch being about 30: a tile takes its sums' steps, or
+// the 9 that its epilogue takes; t1 tiles of s1 steps and then t2 of s2 (Walk).
+constexpr int kLaunchSteps = 30;
+constexpr int kDrainSteps = 9;
+struct LaunchPlan {
+  int64_t steps;
+  int splits, rounds, lead;
+};
+LaunchPlan plan_launch(int64_t t1, int64_t s1, int64_t t2, int64_t s2, const void* kernel, int device) {
+  const int64_t pairs = std::max(device_sm_count(device) / 2, 1), tiles = t1 + t2;
+  const int64_t longest = std::max(t1 ? s1 : 0, t2 ? s2 : 0);
+  LaunchPlan best{};
+  best.splits = split_count(kernel, tiles, longest, device);
+  best.rounds = -1;
+  if (best.splits > 1) {
+    best.steps = kLaunchSteps + kJoinSteps + ceil_div(longest, best.splits);
+    return best;
+  }
+  const int64_t workers = std::min(tiles, pairs), lead = t2 % workers, others = workers - lead;
+  const int64_t c1 = std::max<int64_t>(s1, kDrainSteps), c2 = std::max<int64_t>(s2, kDrainSteps);
+  best.lead = int(lead);
+  // the others' rounds alone: as many as the leading pairs' tiles take, or one or two fewer
+  const int64_t most = lead ? std::min(ceil_div(c2, c1) + 1, ceil_div(t1, others)) : 0;
+  for (int64_t alone = most; alone >= std::max<int64_t>(most - 2, 0); --alone) {
+    const int64_t rounds = ceil_div(std::max<int64_t>(t1 - alone * others, 0), workers);
+    const int64_t steps = kLaunchSteps + t2 / workers * c2 + std::max(alone * c1, lead ? c2 : 0) + rounds * c1;
+    if (best.rounds < 0 || steps < best.steps) {
+      best.steps = steps;
+      best.rounds = int(rounds);
+    }
+  }
+  return best;
+}
+
+// Whether both gradients take less time in one launch.  1000 x 2048 -> 1024: 12 us with one launch, 26 with two.
+bool one_launch(const ProductArgs& p, int device) {
+  const int64_t t1 = most_tiles(kInputGrad, p), s1 = steps_of(kInputGrad, p), t2 = most_tiles(kWeightGrad, p), s2 = steps_of(kWeightGrad, p);
+  const void* kernel = reinterpret_cast<const void*>(kernel_of(kBothGrads, false));
+  return plan_launch(t1, s1, t2, s2, kernel, device).steps <=
+         plan_launch(t1, s1, 0, 0, kernel, device).steps + plan_launch(0, 0, t2, s2, kernel, device).steps;
+}
+
 }  // namespace
 
 int product_status(int* status_out, int clear, cudaStream_t stream) {
@@ -871,37 +941,17 @@ int launch_product(ProductKind kind, const ProductArgs& args, int device, cudaSt
 
   const KernelFn kernel = kernel_of(kind, finish);
   if ((rc = configure(kind, finish, device))) return rc;
-  const int64_t steps = std::max(weight ? 0 : steps_of(kInputGrad, args), weight || both ? steps_of(kWeightGrad, args) : 0);
-  s.splits = split_count(reinterpret_cast<const void*>(kernel), tiles, steps, device);
+  const LaunchPlan plan = plan_launch(weight ? 0 : most_tiles(kInputGrad, args), steps_of(kInputGrad, args),
+                                    weight || both ? most_tiles(kWeightGrad, args) : 0, steps_of(kWeightGrad, args),
+                                    reinterpret_cast<const void*>(kernel), device);
+  s.splits = plan.splits;
+  s.rounds = args.offsets ? -1 : plan.rounds;  // the number of ragged tiles is only a bound here
+  s.lead = plan.lead;
   cudaLaunchAttribute attr[1];
   const cudaLaunchConfig_t cfg = cluster_config(int(std::min(tiles, int64_t(sms / 2))), s.splits, stream, attr);
   MB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps, args, s));
   return kOk;
 }
-
-namespace {
-
-// Whether both gradients take less time in one launch, by their steps (0.27 us): start, epilogue and launch are about 30, and
-// a launch's sums are as long as its longest tile's, split where it is, or as what the busiest pair of CTAs has to do.  1000 x 2048 ->
-// 1024: 12 us with one launch, 26 with two; 16384 x 7168 -> 256, 28 tiles of 256 steps after 1792 of 4: 140 and 127.
-bool one_launch(const ProductArgs& p, int device) {
-  const int64_t pairs = std::max(device_sm_count(device) / 2, 1);
-  const int64_t t1 = most_tiles(kInputGrad, p), s1 = steps_of(kInputGrad, p), t2 = most_tiles(kWeightGrad, p), s2 = steps_of(kWeightGrad, p);
-  auto time = [&](int64_t first, int64_t second) {
-    const int64_t longest = std::max(first ? s1 : 0, second ? s2 : 0);
-    const int splits = split_count(reinterpret_cast<const void*>(kernel_of(kBothGrads, false)), first + second, longest, device);
-    if (splits > 1) return 30 + kJoinSteps + ceil_div(longest, splits);
-    int64_t busiest = 0;
-    for (int64_t i = 0; i < pairs; ++i) {
-      const int64_t mine = ceil_div(std::max(first - i, int64_t(0)), pairs), all = ceil_div(std::max(first + second - i, int64_t(0)), pairs);
-      busiest = std::max(busiest, mine * s1 + (all - mine) * s2);
-    }
-    return 30 + busiest;
-  };
-  return time(t1, t2) <= time(t1, 0) + time(0, t2);
-}
-
-}  // namespace
 
 int launch_gradients(const ProductArgs& args, void* dx, void* dw, int dw_fp32, const void* w, int64_t w_pitch, int64_t w_group,
                      const void* x, int64_t x_pitch, int device, cudaStream_t stream) {

@@ -104,7 +104,8 @@ def test_gradients(rows, k, n, dtype, with_slope):
 
 
 @pytest.mark.parametrize("rows,k,n", [(20, 512, 512), (300, 1024, 1024), (130, 2048, 264), (600, 512, 333), (64, 4096, 64), (2000, 256, 1500),
-                                      (1000, 2048, 1024), (5000, 264, 72), (9000, 256, 520)])
+                                      (1000, 2048, 1024), (5000, 264, 72), (9000, 256, 520), (1500, 2048, 64), (5000, 2048, 72),
+                                      (3000, 1032, 2100)])
 def test_both_gradients_with_sums_of_different_lengths(rows, k, n):
     """In one launch or in two, split or not: dx sums over n, dw over the rows."""
     g = _gen(rows + k)
