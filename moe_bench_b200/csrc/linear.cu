@@ -20,8 +20,9 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // One pass over dy and slope, bound by HBM.  A block takes 32 * kVec columns of a run of rows, 8 rows side by side: a
 // thread has kVec neighbouring columns (16 bytes, or one element where rows do not start on vectors) of every eighth
 // row, four of them requested ahead, and sums them in fp32; the eight are added in order, and the runs' sums by
-// column_sums_kernel, or where there are up to eight runs by the first block of a cluster.  With slope 4096 x 2048 takes 10 us and 8192 x 7168 62 us with both kernels, 1.3 and 1.15 times its
-// bytes at the copy rate (one element per thread in 64 runs: 22 and 236 us).
+// column_sums_kernel, or where there are up to eight runs by the first block of a cluster.  With slope 4096 x 2048 takes 10 us
+// and 8192 x 7168 62 us with both kernels, 1.3 and 1.15 times its bytes at the copy rate (one element per thread in 64 runs:
+// 22 and 236 us).
 constexpr int kRowLanes = 8;
 constexpr int kRowsAhead = 4;
 
