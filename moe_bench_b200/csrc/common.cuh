@@ -468,11 +468,15 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// Both barriers are `.aligned`: a warp arrives on them as one, so whatever branches its lanes took before (and nothing else
+// need have brought them together) they meet here first.
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The same without the order: nobody waits for this thread's global stores, only for its being here.
 __device__ __forceinline__ void cluster_sync_relaxed() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 // Arrival on a barrier of either CTA; orders this thread's earlier accesses before it, cluster-wide.

@@ -168,7 +168,6 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const ProductArgs
       finish4(p.epi, p.m, row, f0 + f, z, vec);
     }
   }
-  __syncwarp();
   if (parts > 1) cluster_sync();  // the other blocks' sums have been read
 }
 

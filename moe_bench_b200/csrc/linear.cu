@@ -116,7 +116,6 @@ __global__ void __launch_bounds__(256, 4) output_grad_kernel(const OutputGrad p)
     else p.sums[int64_t(blockIdx.y) * p.n + at] = t;
   }
   if (!p.joined) return;
-  __syncwarp();
   cluster_sync();
   if (blockIdx.y == 0)
     for (int c = threadIdx.x; c < 32 * kVec; c += 256) {
@@ -130,7 +129,6 @@ __global__ void __launch_bounds__(256, 4) output_grad_kernel(const OutputGrad p)
       }
       p.sums[at] = t;
     }
-  __syncwarp();
   cluster_sync();  // the first block has read the others' sums
 }
 

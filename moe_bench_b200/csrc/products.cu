@@ -285,7 +285,6 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
     ok = mbar_wait(smem_u32(&t->acc_full[0]), 0, ctx, 26);
     tc_fence_after();
   }
-  __syncwarp();
   cluster_sync_relaxed();  // every pair's products have read their stages
   const bool summed = c.step1 > c.step0;
   const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
@@ -308,7 +307,6 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
                      : "memory");
     }
   }
-  __syncwarp();
   cluster_sync();
   if (!ok) return;
   const Output out = output_of(p, shape, kKind == kBothGrads && c.weight);
@@ -761,8 +759,9 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
   // ---------------- teardown ----------------
   __syncwarp();
   tc_fence_before();
-  if (t->abort_flag) {
-    // a wait was abandoned: copies and products still in flight get time to land
+  // a wait was abandoned: copies and products still in flight get time to land (another warp may raise the flag while the
+  // lanes read it)
+  if (__any_sync(0xffffffffu, t->abort_flag)) {
     for (int i = 0; i < 64; ++i) __nanosleep(1000);
   }
   cluster_sync_relaxed();  // the other CTA arrives on this one's barriers no more
