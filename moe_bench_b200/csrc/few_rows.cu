@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const ProductArgs
         b[u][o] = inside ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.b) + x_at[o] + k))
                          : make_uint4(0, 0, 0, 0);
     }
+    __syncwarp();  // in the sum's last chunk not every lane has terms; the products are the whole warp's
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
 #pragma unroll

@@ -316,6 +316,7 @@ __device__ __forceinline__ void join_parts(const ProductArgs& p, const TileShape
     ColumnResidual res{};
     if (kFinish) res = load_residual_column(p.epi, p.m, c, k, f);
     uint32_t v[16];
+    __syncwarp();  // a lane without a feature has not loaded; tensor memory is read by whole warps
     tmem_ld16(lanes + k * 16, v);
     tmem_ld_wait16(v);
     float z[16] = {};
@@ -659,6 +660,7 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
           if (p.epi.residual) request(first_chunk);
         }
         if (!mbar_wait(smem_u32(&t->acc_full[buf]), use & 1, ctx, 25)) break;
+        __syncwarp();  // the loads above are some lanes'; tensor memory is read by whole warps
         tc_fence_after();
         for (int k = first_chunk; k < chunks; k += 4) {
           uint32_t v[2][16];
@@ -738,9 +740,11 @@ product_kernel(const __grid_constant__ Maps maps, const ProductArgs p, const Til
         tc_fence_after();
         for (int k = first_chunk; k < chunks; k += 2) {
           uint32_t v[16];
+          __syncwarp();  // lanes without a feature have neither loaded nor stored
           tmem_ld16(lanes + k * 16, v);
           ColumnResidual next{};
           if (kFinish) next = load_residual_column(p.epi, p.m, c, k + 2, f);
+          __syncwarp();
           tmem_ld_wait16(v);
           if (k + 2 >= chunks) release();
           float z[16];
