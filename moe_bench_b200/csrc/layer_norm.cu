@@ -200,6 +200,7 @@ __device__ __forceinline__ void row_sums(float (&v)[kCount], float (*part)[32][2
   if (lane == 0)
 #pragma unroll
     for (int c = 0; c < kCount; ++c) part[turn][threadIdx.x >> 5][c] = v[c];
+  __syncwarp();  // the barrier is reached by whole warps
   asm volatile("bar.sync %0, %1;" ::"r"(threadIdx.y + 1), "r"(blockDim.x) : "memory");
 #pragma unroll
   for (int c = 0; c < kCount; ++c) v[c] = lane < warps ? part[turn][lane][c] : 0.f;

@@ -80,3 +80,14 @@ def test_a_warp_is_whole_at_the_tensor_cores_registers_and_memory(name):
     assert loops
     for body in loops:
         assert not _split_at(body + body)
+
+
+def test_a_warp_is_whole_at_a_named_barrier():
+    """bar.sync is the aligned form: the statement before each is the one that brings the lanes together."""
+    found = 0
+    for path in glob.glob(os.path.join(mb_build.CSRC, "*.cu*")):
+        text = _source(os.path.basename(path))
+        for m in re.finditer(r'asm volatile\("bar\.sync', text):
+            found += 1
+            assert re.search(r"__syncwarp\(\);\s*$", text[: m.start()]), path
+    assert found
