@@ -100,7 +100,7 @@ template <int kOctets>
 __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const ProductArgs p, int parts, int vec) {
   constexpr int kRows = 8 * kOctets;
   __shared__ float sums[kWarps][kRows][kFeatures];
-  __shared__ float block_sum[kRows][kFeatures];
+  __shared__ __align__(16) float block_sum[kRows][kFeatures];  // read four at a time
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q = lane & 3;
   const int part = int(blockIdx.x) % parts;  // consecutive blocks form a cluster
