@@ -112,7 +112,12 @@ def make_gate(config: MoEBenchConfig) -> GateParams:
 
 def route_hidden(hidden: torch.Tensor, gate: GateParams, topk: int):
     """Layer norm, gate projection with fp32 logits, softmax, top-k, renormalise on the GPU: returns
-    ``(normalised hidden states, ids int32, weights fp32)``, what a ``MoEProblem`` is made of."""
+    ``(normalised hidden states, ids int32, weights fp32)``, what a ``MoEProblem`` is made of.  It runs on the hidden states'
+    device and its current stream."""
+    dev = hidden.get_device()
+    if capi._elsewhere(dev):  # the selection launches on the current device
+        with torch.cuda.device(dev):
+            return route_hidden(hidden, gate, topk)
     x, _, _ = capi.layer_norm(hidden, gate.norm_weight, gate.norm_bias, eps=gate.eps)
     logits = capi.linear(x, gate.weight, bias=gate.bias, out_dtype=torch.float32)
     ids, weights = capi.route_topk(logits, topk)
