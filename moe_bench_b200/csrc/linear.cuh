@@ -64,8 +64,11 @@ __device__ __forceinline__ float load_h16(const void* p, int64_t i, int fp16) {
               : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
 }
 
-// 1 / (1 + exp(-v)): exp and the quotient are good to about 2^-22 of their values plus |v| 2^-24, far inside any 16-bit
-// rounding and about 2 units of an fp32 output.
+// 1 / (1 + exp(-v)), with an error that grows with |v| where v is negative, since the exponential's argument is rounded: at
+// most (9 + 2.35 |v|) 2^-24 of the value by CUDA's bounds of __expf and __fdividef, for v >= 0 9 of them.  Measured with an fp32
+// output, SiLU is off by 3.5 steps of 2^-24 from z = -1 up, 9 at -10, 18 at -20 and 65 at -87; GELU's tanh form, whose argument is a
+// polynomial, by 5 from -1 up, 47 at -5 and 255 at -10.  All of it is far inside a 16-bit rounding (2^-11 and 2^-8).  Below
+// v = -87.3 the divisor is past 2^126 and the quotient 0 instead of less than 2^-126: SiLU is -0 there where up to -1e-36 is meant.
 __device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 
 // The normal distribution's mass beyond |z|, 1 - Phi(|z|), over exp(-z^2 / 2): u P(u) with u = 1 / (1 + 0.28 |z|), where P is a
