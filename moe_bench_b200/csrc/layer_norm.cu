@@ -680,7 +680,8 @@ Plan make_plan(bool backward, int elem_bytes, bool aligned, int64_t rows, int64_
   l.per = s.per;
   l.most = s.most;
   const int tpr = int((vecs + l.per - 1) / l.per + 31) / 32 * 32;
-  // Rows of one warp go eight to a block; backward, where a block leaves sums for a second kernel to add, also rows of up to four
+  // Rows of one warp go side by side, as many as the shape has threads for, up to eight (forward two with many rows, whose blocks
+  // have 64 threads; eight with few); backward, where a block leaves sums for a second kernel to add, also rows of up to four
   // warps, side by side (10000 rows of 1536: 31 -> 21 us, 3000 of 1024 13.7 -> 9.5; of eight warps 19.6 -> 21.1, so not there)
   const bool side_by_side = tpr == 32 || (backward && !few && tpr <= 128);
   l.block = dim3(tpr, side_by_side ? std::min(kMostRows, s.most / tpr) : 1);
@@ -700,7 +701,7 @@ KernelFn forward_kernel(const Plan& l) {
   if (l.vec == 0) return norm_long_kernel<T>;
   if (l.vec == 1) return l.per == 4 ? norm_kernel<T, 1, 4, 1024, 1> : norm_kernel<T, 1, 16, 1024, 1>;
   if (l.per == 1) return norm_kernel<T, kV, 1, 1024, 1>;
-  return l.per == 2 ? norm_kernel<T, kV, 2, 256, 4> : norm_kernel<T, kV, 4, 512, 1>;
+  return l.per == 2 ? norm_kernel<T, kV, 2, 64, 16> : norm_kernel<T, kV, 4, 512, 1>;
 }
 template <typename T>
 KernelFn backward_kernel(const Plan& l) {
