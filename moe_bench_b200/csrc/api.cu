@@ -72,6 +72,20 @@ EncodeTiledFn encode_tiled_fn() {
   }();
   return fn;
 }
+
+// Encodes a map.  The driver's call needs a context, which a host thread that has made no runtime call yet (one of autograd's, a
+// server's worker) does not have, even where its tensors lie on the device: the thread's device is then set, which binds it.
+CUresult encode_tiled(EncodeTiledFn fn, CUtensorMap* map, CUtensorMapDataType type, uint32_t rank, const void* base, const cuuint64_t* dims,
+                      const cuuint64_t* strides, const cuuint32_t* box, const cuuint32_t* elem_strides) {
+  auto encode = [&] {
+    return fn(map, type, rank, const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  int device;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess) r = encode();
+  return r;
+}
 }  // namespace
 
 int make_tensor_map_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t rows,
@@ -92,9 +106,7 @@ int make_tensor_map_2d(CUtensorMap* map, const void* base, int elem_bytes, uint6
   const CUtensorMapDataType dtype = elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                     : fp16          ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  CUresult r = fn(map, dtype, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode_tiled(fn, map, dtype, 2, base, dims, strides, box, estr);
   MB200_REQUIRE(r == CUDA_SUCCESS, kCudaError, "cuTensorMapEncodeTiled failed with code %d", int(r));
   return kOk;
 }
@@ -114,9 +126,8 @@ int make_tensor_map_3d(CUtensorMap* map, const void* base, uint64_t cols, uint64
   const cuuint64_t strides[2] = {row_bytes, group_bytes};
   const cuuint32_t box[3] = {64, box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
-                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = encode_tiled(fn, map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides,
+                                  box, estr);
   MB200_REQUIRE(r == CUDA_SUCCESS, kCudaError, "cuTensorMapEncodeTiled failed with code %d", int(r));
   return kOk;
 }
