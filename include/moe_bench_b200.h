@@ -373,8 +373,9 @@ int mb200_linear(int precision, const void* x, int64_t x_pitch, int64_t rows, co
  * [n], from dz before any rounding.  Each of dx, dw, db may be NULL.  dy [rows, n] is fp32 if
  * dy_fp32 (bf16 only: the range of fp16 does not hold such a gradient).  The products take dz in
  * the precision's type: where slope is given or dy is fp32 it is rounded to it once, into the
- * workspace (in fp16 a dy of 65504 times a slope above 1 is infinite there), and a dy that breaks the alignment rules (n odd, say) is copied there too: copies_dy
- * of the query says that one of these is so.  Else the workspace holds the parts of db alone. */
+ * workspace (in fp16 a dy of 65504 times a slope above 1 is infinite there), and a dy that breaks
+ * the alignment rules (n odd, say) is copied there too: copies_dy of the query says that one of
+ * these is so.  Else the workspace holds the parts of db alone. */
 int64_t mb200_linear_backward_workspace_bytes(int64_t rows, int n, int copies_dy, int device);
 int mb200_linear_backward(int precision, const void* dy, int dy_fp32, int64_t dy_pitch, const void* slope,
                           const void* x, int64_t x_pitch, int64_t rows, const void* w, int64_t w_pitch, int n,

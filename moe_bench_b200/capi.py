@@ -505,6 +505,8 @@ def read_kernel_clocks(workspace: torch.Tensor) -> dict:
 
 # ---- products and norms around the expert FFN ----
 # The tensors of these calls may be on any device: the call runs there, on that device's current stream.
+# They stand outside autograd: a result carries no graph, whether or not an operand requires gradients.  A program that trains
+# makes the backward calls itself, or from a torch.autograd.Function of its own.
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 _H16 = {torch.bfloat16: PRECISION_BF16, torch.float16: PRECISION_FP16}

@@ -67,3 +67,29 @@ def test_first_call_of_a_thread(name):
     torch.cuda.synchronize()
     assert not isinstance(got[0], Exception), got[0]
     assert all(torch.equal(a, b) for a, b in zip(got[0], expect))
+
+
+def test_first_call_of_a_thread_into_a_capture():
+    """The stream is being captured by another thread, in the mode that is strictest about what others call."""
+    x, w = _operands()[:2]
+    expect, failed = capi.linear(x, w), []
+    out = torch.zeros_like(expect)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        stream = torch.cuda.current_stream()
+
+        def work():
+            try:
+                with torch.cuda.stream(stream):
+                    capi.linear(x, w, out=out)
+            except Exception as e:
+                failed.append(e)
+
+        thread = threading.Thread(target=work)
+        thread.start()
+        thread.join()
+    assert not failed, failed[0]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, expect)
